@@ -1,0 +1,575 @@
+// Linear selective log-softmax: log-probabilities of given tokens from hidden
+// states and the head's weight, and the gradients of both for any gradient of
+// the log-probabilities, without the [N, V] logits.
+//
+//   x[r, v] = (H[r] . W[v]) / temperature       y[r] = x[r, t] - log sum_v e^x[r, v]
+//   d[r, v] = g[r] / temperature * ([v = t] - e^(x[r, v] - lse[r]))
+//   dH = d W        dW = d^T H
+//
+// The forward is one logits GEMM whose epilogue keeps (max, sum of
+// exponentials) per row and 256-column tile and the target's logit, all from
+// the fp32 accumulator (tc_gemm.cuh, EPI_LSM); a combine kernel merges the
+// tiles, with the last logarithm and the difference in fp64, which costs
+// nothing per row.
+//
+// Two backward forms:
+//   kept       (bf16) the forward's epilogue also stores q = e^x in 16 bits. With
+//              a[r] = -g[r] / temperature * e^-lse[r], d = a (q - e^lse onehot):
+//              the one-hot part goes into q's target column, a into dH's epilogue
+//              and into a 16-bit copy of H for dW. Three GEMMs for both passes.
+//   recomputed the backward repeats the logits GEMM row chunk by row chunk with an
+//              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, 2 GB of
+//              workspace whatever N, and fp16 (whose exponent cannot hold e^x).
+// Bound by the tensor pipe for many rows and by reading W once for few.
+#include "row_ops.cuh"
+#include "tc_gemm_host.cuh"
+
+namespace gh {
+namespace {
+
+inline size_t al256(size_t x) { return (x + 255) & ~size_t(255); }
+
+constexpr double kLn2d = 0.6931471805599453;
+constexpr double kLog2ed = 1.4426950408889634;
+
+// ---------------------------------------------------------------------------
+// Row kernels
+
+// Clean targets: -1 for a row that is left out, -2 for an index outside
+// [0, V) (flagged; its log-probability is NaN and it has no gradient).
+template <typename I>
+__global__ void __launch_bounds__(256)
+lsm_targets_kernel(const I* __restrict__ index, int64_t rows, int64_t V, int64_t ignore, int* __restrict__ tgt,
+                   int* status) {
+  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (r >= rows) return;
+  const int64_t t = (int64_t)index[r];
+  const bool skip = t == ignore, bad = !skip && (t < 0 || t >= V);
+  if (bad) atomicOr(status, GH_DEV_BAD_LABEL);
+  tgt[r] = skip ? -1 : bad ? -2 : (int)t;
+}
+
+struct CombineOut {
+  float* y;        // [rows] log-probability of the target (0: left out)
+  float* lse2;     // [rows] log-sum-exp, log2 units (may be NULL)
+  // kept form only (q == NULL otherwise)
+  __nv_bfloat16* q;
+  int64_t ldq;
+  const uint8_t* qmode;
+  float* alpha0;   // [rows] factor that turns the stored row into p - onehot; 0: left out
+  int* rowflag;    // [rows] 1: rewrite the row, 2: zero it
+};
+
+// Merge the per-tile (max, sum) pairs of TR rows per block. TR = 32 reads
+// 32 rows x 8 tiles at a time (coalesced: the partials are [tile][row]); few
+// rows take TR = 1, 256 tiles at a time, whose strided reads cost less than
+// the 63 dependent steps of 8 warps over a 128256-column vocabulary.
+template <int TR>
+__global__ void __launch_bounds__(256)
+lsm_combine_kernel(const float2* __restrict__ stats, int num_n, int64_t rows, int64_t V, float sc2,
+                   const float* __restrict__ xt, const int* __restrict__ tgt, CombineOut o) {
+  constexpr int SL = 256 / TR;
+  __shared__ float sm[256], ss[256];
+  __shared__ int sf[256];
+  const int tid = threadIdx.x, slice = tid / TR;
+  const int64_t r = (int64_t)blockIdx.x * TR + tid % TR;
+  MS acc = ms_empty();
+  int flag = 0;
+  if (r < rows) {
+#pragma unroll 4
+    for (int j = slice; j < num_n; j += SL) {
+      const float2 p = stats[(int64_t)j * rows + r];
+      acc = ms_merge(acc, MS{p.x, p.y});
+      if (o.q) {
+        flag |= o.qmode[((int64_t)j * 2) * rows + r];
+        if ((int64_t)j * BN + BN / 2 < V) flag |= o.qmode[((int64_t)j * 2 + 1) * rows + r];
+      }
+    }
+  }
+  sm[tid] = acc.m;
+  ss[tid] = acc.s;
+  sf[tid] = flag;
+  __syncthreads();
+#pragma unroll
+  for (int s = SL / 2; s > 0; s >>= 1) {
+    if (slice < s) {
+      const MS t = ms_merge(MS{sm[tid], ss[tid]}, MS{sm[tid + s * TR], ss[tid + s * TR]});
+      sm[tid] = t.m;
+      ss[tid] = t.s;
+      sf[tid] |= sf[tid + s * TR];
+    }
+    __syncthreads();
+  }
+  if (slice != 0 || r >= rows) return;
+  const double lse2 = (double)sm[tid] + log2((double)ss[tid]);
+  const int t = tgt[r];
+  double y = t >= 0 ? kLn2d * ((double)xt[r] * (double)sc2 - lse2) : 0.0;
+  if (y > 0.0) y = 0.0;  // rounding at p = 1; a NaN stays
+  o.y[r] = t == -2 ? __int_as_float(0x7fc00000) : (float)y;
+  if (o.lse2) o.lse2[r] = (float)lse2;
+  if (!o.q) return;
+  const bool odd = sf[tid] || !(lse2 >= (double)gemm::kLsmQLo && lse2 <= (double)gemm::kLsmQHi + 32.0);
+  if (t < 0) {
+    // a left-out row must not reach the gradients, not even as 0 * NaN
+    o.alpha0[r] = 0.f;
+    o.rowflag[r] = odd ? 2 : 0;
+    return;
+  }
+  // The target's entry of p - onehot is -(1 - p_t) = expm1(y); it outweighs
+  // its row. Its 16-bit rounding would reach dW on top of the one of a * H, so
+  // the row factor takes it out: alpha0 * (stored target) is exact to fp32, and
+  // the row's other entries, each rounded already, move by at most 2^-9.
+  const double tau = expm1(y) * (odd ? 1.0 : exp2(lse2));
+  const __nv_bfloat16 c = __float2bfloat16_rn((float)tau);
+  const double cd = (double)__bfloat162float(c);
+  const double fix = cd != 0.0 ? tau / cd : 1.0;
+  o.alpha0[r] = (float)((odd ? 1.0 : exp2(-lse2)) * fix);
+  o.rowflag[r] = odd ? 1 : 0;
+  if (!odd) o.q[r * o.ldq + t] = c;
+}
+
+// Rewrite the rows that q cannot represent (a group outside the exponent
+// window, a log-sum-exp outside it) as p - onehot, and zero left-out rows
+// whose values are no fit operand. Most rows return at once.
+__global__ void __launch_bounds__(256)
+lsm_fixup_kernel(__nv_bfloat16* q, int64_t ld, const uint8_t* __restrict__ qmode, const float* __restrict__ gmax,
+                 const int* __restrict__ rowflag, const float* __restrict__ lse2, const float* __restrict__ y,
+                 const int* __restrict__ tgt, int64_t rows, int64_t V) {
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int f = rowflag[row];
+    if (!f) continue;
+    __nv_bfloat16* yq = q + row * ld;
+    const int t = tgt[row];
+    const float l2 = lse2[row];
+    for (int64_t c = threadIdx.x; c < V; c += 256) {
+      float v = 0.f;
+      if (f == 1) {
+        const int64_t grp = ((c >> 8) * 2 + ((c >> 7) & 1)) * rows + row;
+        const float stored = __bfloat162float(yq[c]);
+        const float up = (qmode[grp] ? gmax[grp] : 0.f) - l2;
+        // 2^up alone may overflow or vanish where the product does not
+        v = stored > 0.f ? fast_exp2(fast_log2(stored) + up) : stored;
+        if (up != up) v = up;  // a log-sum-exp of NaN: the row's gradient is NaN
+        if (c == t) v = expm1f(y[row]);
+      }
+      yq[c] = __float2bfloat16_rn(v);
+    }
+  }
+}
+
+// Backward, kept form: a[r] = -g[r] / temperature * alpha0[r] and a * H in 16
+// bits, the dW GEMM's second operand (its rounding is dW's only one before
+// the output's). Left-out rows give exact zeros.
+__global__ void __launch_bounds__(256)
+lsm_rows_kernel(const __nv_bfloat16* __restrict__ H, const float* __restrict__ g, const float* __restrict__ alpha0,
+                float inv_t, int64_t rows, int64_t D, float* __restrict__ a_out, __nv_bfloat16* __restrict__ hs) {
+  const int64_t vpr = D / 8, n = rows * vpr;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / vpr;
+    const float a0 = alpha0[r];
+    const float a = a0 == 0.f ? 0.f : -g[r] * inv_t * a0;
+    if (i - r * vpr == 0) a_out[r] = a;
+    if (!hs) continue;
+    Vec16<__nv_bfloat16> v;
+    if (a0 == 0.f) {
+      v.raw = make_uint4(0, 0, 0, 0);
+    } else {
+      v.raw = ld16(reinterpret_cast<const uint4*>(H) + i);
+      float f[8];
+      v.to_float(f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= a;
+      v.from_float(f);
+    }
+    st16(reinterpret_cast<uint4*>(hs) + i, v.raw);
+  }
+}
+
+// Backward, recomputed form, fp16: d is written times 2^k so that the largest
+// row factor lies in [2^13, 2^14): (onehot - p) keeps 2^-38 of the largest
+// gradient instead of fp16's 2^-24. scale = {2^k, 2^-k}; non-finite gradients
+// do not count.
+__global__ void __launch_bounds__(1024)
+lsm_gscale_kernel(const float* __restrict__ g, const int* __restrict__ tgt, int64_t rows, float inv_t, float* scale) {
+  __shared__ float sm[32];
+  float m = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    const float v = fabsf(g[r] * inv_t);
+    if (tgt[r] >= 0 && v <= 3.4e38f) m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 32; ++i) m = fmaxf(m, sm[i]);
+    int k = 0;
+    if (m > 0.f) k = 13 - ilogbf(m);
+    k = k < -120 ? -120 : k > 120 ? 120 : k;  // both powers stay normal
+    scale[0] = ldexpf(1.f, k);
+    scale[1] = ldexpf(1.f, -k);
+  }
+}
+
+// Row factor and target value of EPI_LSM_GRAD for all rows.
+__global__ void __launch_bounds__(256)
+lsm_factor_kernel(const float* __restrict__ g, const float* __restrict__ y, const int* __restrict__ tgt, float inv_t,
+                  const float* __restrict__ scale, int64_t rows, float* __restrict__ rfac, float* __restrict__ tval) {
+  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (r >= rows) return;
+  const float f = tgt[r] >= 0 ? g[r] * inv_t * (scale ? scale[0] : 1.f) : 0.f;
+  rfac[r] = f;
+  tval[r] = tgt[r] >= 0 ? -f * expm1f(y[r]) : 0.f;
+}
+
+// H with left-out rows zeroed (0 * NaN must not reach dW): the dW GEMM's second
+// operand in the recomputed form.
+__global__ void __launch_bounds__(256)
+lsm_clean_rows_kernel(const uint4* __restrict__ H, const int* __restrict__ tgt, int64_t rows, int64_t vpr,
+                      uint4* __restrict__ out) {
+  const int64_t n = rows * vpr;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    st16(out + i, tgt[i / vpr] >= 0 ? ld16(H + i) : make_uint4(0, 0, 0, 0));
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+
+struct FwdLayout {
+  size_t status = 0, tgt, xt, lse2, rowflag, stats, qmode, gmax, total;
+  int64_t chunk;
+  int num_n;
+};
+
+// keep: one chunk of all rows (the stored q is one operand of the backward).
+FwdLayout fwd_layout(int64_t N, int64_t V, int64_t chunk, bool keep) {
+  FwdLayout L;
+  if (keep || chunk <= 0 || chunk > N) chunk = N;
+  L.chunk = chunk;
+  L.num_n = (int)((V + BN - 1) / BN);
+  size_t off = 256;
+  L.tgt = off;     off = al256(off + sizeof(int) * N);
+  L.xt = off;      off = al256(off + sizeof(float) * chunk);
+  L.lse2 = off;    off = al256(off + sizeof(float) * N);
+  L.rowflag = off; off = al256(off + sizeof(int) * (keep ? N : 0));
+  L.stats = off;   off = al256(off + sizeof(float2) * (size_t)L.num_n * chunk);
+  L.qmode = off;   off = al256(off + (keep ? (size_t)L.num_n * 2 * chunk : 0));
+  L.gmax = off;    off = al256(off + (keep ? sizeof(float) * (size_t)L.num_n * 2 * chunk : 0));
+  L.total = off;
+  return L;
+}
+
+// What the kept form holds between the passes: q and the row factors.
+struct KeptLayout {
+  size_t q = 0, alpha0, total;
+  int64_t ldq;
+};
+KeptLayout kept_layout(int64_t N, int64_t V) {
+  KeptLayout L;
+  L.ldq = (V + 7) / 8 * 8;  // 16-byte row pitch for TMA
+  size_t off = al256((size_t)N * L.ldq * 2);
+  L.alpha0 = off;
+  off = al256(off + sizeof(float) * N);
+  L.total = off;
+  return L;
+}
+
+struct BwdLayout {
+  size_t status = 0, scale = 64, tgt, rfac, tval, d, hs, dh2, acc, total;
+  int64_t chunk, ldd;
+  bool need_acc;
+};
+BwdLayout bwd_layout(int64_t N, int64_t D, int64_t V, int64_t chunk, bool kept, bool fp32_accum) {
+  BwdLayout L;
+  if (kept || chunk <= 0 || chunk > N) chunk = N;
+  L.chunk = chunk;
+  L.ldd = (V + 7) / 8 * 8;
+  size_t off = 256;
+  L.tgt = off;  off = al256(off + (kept ? 0 : sizeof(int) * N));
+  L.rfac = off; off = al256(off + sizeof(float) * N);  // kept: a
+  L.tval = off; off = al256(off + (kept ? 0 : sizeof(float) * N));
+  L.d = off;    off = al256(off + (kept ? 0 : (size_t)chunk * L.ldd * 2));
+  L.hs = off;   off = al256(off + (size_t)chunk * D * 2);
+  L.dh2 = off;  off = al256(off + (size_t)chunk * D * 2);
+  L.need_acc = !kept && fp32_accum && N > chunk;
+  L.acc = off;
+  if (L.need_acc) off = al256(off + sizeof(float) * (size_t)D * V);
+  L.total = off;
+  return L;
+}
+
+int targets(const void* index, int index_dtype, int64_t N, int64_t V, int64_t ignore, int* tgt, int* status,
+            cudaStream_t st) {
+  const unsigned grid = (unsigned)((N + 255) / 256);
+  if (index_dtype == GH_I64)
+    lsm_targets_kernel<int64_t><<<grid, 256, 0, st>>>(static_cast<const int64_t*>(index), N, V, ignore, tgt, status);
+  else
+    lsm_targets_kernel<int32_t><<<grid, 256, 0, st>>>(static_cast<const int32_t*>(index), N, V, ignore, tgt, status);
+  count_launch(1);
+  return check_launch("lsm_targets");
+}
+
+// One logits GEMM with a log-probability epilogue over `rows` rows.
+template <typename T, int EPI>
+int logits_gemm(const void* H, const void* W, int64_t rows, int64_t D, int64_t V, int dtype, gemm::Params& p,
+                cudaStream_t st) {
+  const int pair = pick_pair(rows);
+  CUtensorMap ta, tb;
+  int rc = make_operand_maps(&ta, &tb, dtype, Operand{H, D, 0}, Operand{W, D, 0}, rows, V, D, pair);
+  if (rc) return rc;
+  set_tiles(p, rows, V, D, pair, 1);
+  p.raster = 2;
+  p.group = logits_group();
+  p.a_hint = kKeepA_StreamB.a;
+  p.b_hint = kKeepA_StreamB.b;
+  p.out_evict_first = kKeepA_StreamB.out;
+  ProfScope prof(PROF_GEMM_LOGITS_CE, st);
+  if (pair == 2) return launch_gemm_t<T, 0, 0, EPI, T, 2>(ta, tb, p, num_sms_dev(), st);
+  return launch_gemm_t<T, 0, 0, EPI, T, 1>(ta, tb, p, num_sms_dev(), st);
+}
+
+int check_common(int64_t N, int64_t D, int64_t V, int dtype, int index_dtype, double inv_t) {
+  if (dtype != GH_BF16 && dtype != GH_F16)
+    return set_error(GH_ETYPE, "expected bf16 or fp16 operands (dtype code %d)", dtype);
+  if (index_dtype != GH_I32 && index_dtype != GH_I64)
+    return set_error(GH_ETYPE, "expected int32 or int64 index, got dtype code %d", index_dtype);
+  if (N < 0 || D <= 0 || V <= 0 || N > INT32_MAX || V > INT32_MAX || D > INT32_MAX)
+    return set_error(GH_EINVAL, "bad shape N=%lld D=%lld V=%lld", (long long)N, (long long)D, (long long)V);
+  if (D % 8) return set_error(GH_EINVAL, "hidden size must be a multiple of 8 (got %lld)", (long long)D);
+  if (!(inv_t > 0.0) || !(inv_t < 1e30)) return set_error(GH_EINVAL, "temperature must be positive and finite");
+  return GH_OK;
+}
+
+template <typename T>
+int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, int dtype, float sc2,
+                const FwdLayout& L, char* kept, float* y, float* lse2_out, char* ws, cudaStream_t st) {
+  int* status = reinterpret_cast<int*>(ws + L.status);
+  int* tgt = reinterpret_cast<int*>(ws + L.tgt);
+  float* lse2 = lse2_out ? lse2_out : reinterpret_cast<float*>(ws + L.lse2);
+  float* xt = reinterpret_cast<float*>(ws + L.xt);
+  float2* stats = reinterpret_cast<float2*>(ws + L.stats);
+  const KeptLayout K = kept_layout(N, V);
+  int rc;
+  for (int64_t s0 = 0; s0 < N; s0 += L.chunk) {
+    const int64_t rows = s0 + L.chunk <= N ? L.chunk : N - s0;
+    gemm::Params p{};
+    p.tgt = tgt + s0;
+    p.sc2 = sc2;
+    p.stats = stats;
+    p.xt = xt;
+    p.status = status;
+    CombineOut o{};
+    o.y = y + s0;
+    o.lse2 = lse2 + s0;
+    const void* Hc = static_cast<const T*>(H) + s0 * D;
+    if constexpr (sizeof(T) == 2 && gemm::AbType<T>::v == 1) {
+      if (kept) {
+        p.out = kept + K.q;
+        p.ldo = K.ldq;
+        p.vec_ok = 1;
+        p.qmode = reinterpret_cast<uint8_t*>(ws + L.qmode);
+        p.gmax = reinterpret_cast<float*>(ws + L.gmax);
+        o.q = reinterpret_cast<__nv_bfloat16*>(kept + K.q);
+        o.ldq = K.ldq;
+        o.qmode = p.qmode;
+        o.alpha0 = reinterpret_cast<float*>(kept + K.alpha0);
+        o.rowflag = reinterpret_cast<int*>(ws + L.rowflag);
+        if ((rc = logits_gemm<T, gemm::EPI_LSM_Q>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+      }
+    }
+    if (!kept && (rc = logits_gemm<T, gemm::EPI_LSM>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+    if (rows <= 4 * (int64_t)num_sms_dev())
+      lsm_combine_kernel<1><<<(unsigned)rows, 256, 0, st>>>(stats, L.num_n, rows, V, sc2, xt, tgt + s0, o);
+    else
+      lsm_combine_kernel<32><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(stats, L.num_n, rows, V, sc2, xt, tgt + s0,
+                                                                          o);
+    count_launch(1);
+    if ((rc = check_launch("lsm_combine"))) return rc;
+    if (kept) {
+      const int64_t cap = 8 * (int64_t)num_sms_dev();
+      lsm_fixup_kernel<<<(unsigned)(rows < cap ? rows : cap), 256, 0, st>>>(o.q, o.ldq, o.qmode, p.gmax, o.rowflag,
+                                                                           o.lse2, o.y, tgt, rows, V);
+      count_launch(1);
+      if ((rc = check_launch("lsm_fixup"))) return rc;
+    }
+  }
+  return publish_status(status, st);
+}
+
+int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V, float inv_t,
+                     const char* kept, void* dH, void* dW, const BwdLayout& L, char* ws, cudaStream_t st) {
+  int* status = reinterpret_cast<int*>(ws + L.status);
+  const KeptLayout K = kept_layout(N, V);
+  const int sms = num_sms_dev();
+  float* a = reinterpret_cast<float*>(ws + L.rfac);
+  __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(ws + L.hs);
+  lsm_rows_kernel<<<4 * sms, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(H), grad,
+                                           reinterpret_cast<const float*>(kept + K.alpha0), inv_t, N, D, a,
+                                           dW ? hs : nullptr);
+  count_launch(1);
+  int rc = check_launch("lsm_rows");
+  if (rc) return rc;
+  if (dW && (rc = run_gemm(GH_BF16, Operand{kept + K.q, K.ldq, 1}, Operand{hs, D, 1}, V, D, N, dW, GH_BF16, D, nullptr,
+                           nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
+    return rc;
+  if (dH && (rc = run_gemm(GH_BF16, Operand{kept + K.q, K.ldq, 0}, Operand{W, D, 1}, N, D, V, dH, GH_BF16, D, nullptr,
+                           nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DH, Hints{}, ws + L.dh2, a)))
+    return rc;
+  return publish_status(status, st);
+}
+
+template <typename T>
+int lsm_bwd_run(const void* H, const void* W, const float* y, const float* lse2, const float* grad, int64_t N,
+                int64_t D, int64_t V, int dtype, float inv_t, float sc2, void* dH, void* dW, bool fp32_accum,
+                const BwdLayout& L, char* ws, cudaStream_t st) {
+  int* status = reinterpret_cast<int*>(ws + L.status);
+  int* tgt = reinterpret_cast<int*>(ws + L.tgt);
+  float* rfac = reinterpret_cast<float*>(ws + L.rfac);
+  float* tval = reinterpret_cast<float*>(ws + L.tval);
+  float* acc = reinterpret_cast<float*>(ws + L.acc);
+  T* d = reinterpret_cast<T*>(ws + L.d);
+  T* hs = reinterpret_cast<T*>(ws + L.hs);
+  const int sms = num_sms_dev();
+  const float* scale = nullptr;
+  if (dtype == GH_F16) {
+    float* s = reinterpret_cast<float*>(ws + L.scale);
+    lsm_gscale_kernel<<<1, 1024, 0, st>>>(grad, tgt, N, inv_t, s);
+    count_launch(1);
+    scale = s;
+  }
+  lsm_factor_kernel<<<(unsigned)((N + 255) / 256), 256, 0, st>>>(grad, y, tgt, inv_t, scale, N, rfac, tval);
+  count_launch(1);
+  int rc = check_launch("lsm_factor");
+  if (rc) return rc;
+  const float* unscale = scale ? scale + 1 : nullptr;
+  for (int64_t s0 = 0; s0 < N; s0 += L.chunk) {
+    const int64_t rows = s0 + L.chunk <= N ? L.chunk : N - s0;
+    const bool first = s0 == 0, last = s0 + rows >= N;
+    const T* Hc = static_cast<const T*>(H) + s0 * D;
+    gemm::Params p{};
+    p.tgt = tgt + s0;
+    p.sc2 = sc2;
+    p.lse2 = lse2 + s0;
+    p.rfac = rfac + s0;
+    p.tval = tval + s0;
+    p.out = d;
+    p.ldo = L.ldd;
+    p.vec_ok = 1;
+    p.status = status;
+    if ((rc = logits_gemm<T, gemm::EPI_LSM_GRAD>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+    if (dW) {
+      lsm_clean_rows_kernel<<<4 * sms, 256, 0, st>>>(reinterpret_cast<const uint4*>(Hc), tgt + s0, rows, D / 8,
+                                                     reinterpret_cast<uint4*>(hs));
+      count_launch(1);
+      if ((rc = check_launch("lsm_clean_rows"))) return rc;
+      void* out = dW;
+      int out_dtype = dtype;
+      const float* add_f32 = nullptr;
+      const void* add_same = nullptr;
+      if (L.need_acc) {
+        out = last ? dW : (void*)acc;
+        out_dtype = last ? dtype : GH_F32;
+        add_f32 = first ? nullptr : acc;
+      } else if (!fp32_accum) {
+        add_same = first ? nullptr : dW;
+      }
+      if ((rc = run_gemm(dtype, Operand{d, L.ldd, 1}, Operand{hs, D, 1}, V, D, rows, out, out_dtype, D, add_f32,
+                         add_same, D, unscale, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
+        return rc;
+    }
+    if (dH && (rc = run_gemm(dtype, Operand{d, L.ldd, 0}, Operand{W, D, 1}, rows, D, V, static_cast<T*>(dH) + s0 * D,
+                             dtype, D, nullptr, nullptr, 0, unscale, 1, sms, st, status, PROF_GEMM_DH, Hints{},
+                             ws + L.dh2)))
+      return rc;
+  }
+  return publish_status(status, st);
+}
+
+}  // namespace
+}  // namespace gh
+
+using namespace gh;
+
+extern "C" size_t gh_lsm_kept_bytes(int64_t N, int64_t V) {
+  return N < 0 || V <= 0 ? 0 : kept_layout(N, V).total;
+}
+
+extern "C" size_t gh_lsm_fwd_workspace_bytes(int64_t N, int64_t V, int64_t chunk_rows, int keep) {
+  return N < 0 || V <= 0 ? 0 : fwd_layout(N, V, chunk_rows, keep != 0).total;
+}
+
+extern "C" size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t chunk_rows, int kept,
+                                             int fp32_grad_weight_accum) {
+  return N < 0 || D <= 0 || V <= 0 ? 0 : bwd_layout(N, D, V, chunk_rows, kept != 0, fp32_grad_weight_accum).total;
+}
+
+extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int index_dtype, int64_t N, int64_t D,
+                          int64_t V, int dtype, int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
+                          float* logprobs, float* lse2, void* kept, size_t kept_bytes, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  int rc = check_common(N, D, V, dtype, index_dtype, inv_temperature);
+  if (rc) return rc;
+  if (N == 0) return GH_OK;
+  if (!H || !W || !index || !logprobs || !workspace) return set_error(GH_EINVAL, "null pointer argument");
+  if (kept && dtype != GH_BF16) return set_error(GH_EUNSUPPORTED, "only bf16 operands keep e^x");
+  if (kept && kept_bytes < kept_layout(N, V).total) return set_error(GH_EWORKSPACE, "kept buffer too small");
+  const FwdLayout L = fwd_layout(N, V, chunk_rows, kept != nullptr);
+  if (workspace_bytes < L.total)
+    return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const float sc2 = (float)(inv_temperature * kLog2ed);
+  int* status = reinterpret_cast<int*>(ws + L.status);
+  cudaMemsetAsync(status, 0, sizeof(int), st);
+  if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
+  char* kp = static_cast<char*>(kept);
+  if (dtype == GH_BF16) return lsm_fwd_run<__nv_bfloat16>(H, W, N, D, V, dtype, sc2, L, kp, logprobs, lse2, ws, st);
+  return lsm_fwd_run<__half>(H, W, N, D, V, dtype, sc2, L, nullptr, logprobs, lse2, ws, st);
+}
+
+extern "C" int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V,
+                               int dtype, double inv_temperature, const void* kept, size_t kept_bytes,
+                               void* grad_input, void* grad_weight, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  int rc = check_common(N, D, V, dtype, GH_I64, inv_temperature);
+  if (rc) return rc;
+  if (dtype != GH_BF16) return set_error(GH_EUNSUPPORTED, "only bf16 operands keep e^x");
+  if (N == 0) return GH_OK;
+  if (!H || !W || !grad || !kept || !workspace) return set_error(GH_EINVAL, "null pointer argument");
+  if (kept_bytes < kept_layout(N, V).total) return set_error(GH_EWORKSPACE, "kept buffer too small");
+  const BwdLayout L = bwd_layout(N, D, V, N, true, true);
+  if (workspace_bytes < L.total)
+    return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  cudaMemsetAsync(ws + L.status, 0, sizeof(int), st);
+  return lsm_bwd_kept_run(H, W, grad, N, D, V, (float)inv_temperature, static_cast<const char*>(kept), grad_input,
+                          grad_weight, L, ws, st);
+}
+
+extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* logprobs,
+                          const float* lse2, const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
+                          int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
+                          int fp32_grad_weight_accum, void* grad_input, void* grad_weight, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  int rc = check_common(N, D, V, dtype, index_dtype, inv_temperature);
+  if (rc) return rc;
+  if (N == 0) return GH_OK;
+  if (!H || !W || !index || !logprobs || !lse2 || !grad || !workspace)
+    return set_error(GH_EINVAL, "null pointer argument");
+  const BwdLayout L = bwd_layout(N, D, V, chunk_rows, false, fp32_grad_weight_accum);
+  if (workspace_bytes < L.total)
+    return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const float inv_t = (float)inv_temperature;
+  const float sc2 = (float)(inv_temperature * kLog2ed);
+  int* status = reinterpret_cast<int*>(ws + L.status);
+  cudaMemsetAsync(status, 0, sizeof(int), st);
+  if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
+  if (dtype == GH_BF16)
+    return lsm_bwd_run<__nv_bfloat16>(H, W, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, grad_input, grad_weight,
+                                      fp32_grad_weight_accum, L, ws, st);
+  return lsm_bwd_run<__half>(H, W, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, grad_input, grad_weight,
+                             fp32_grad_weight_accum, L, ws, st);
+}

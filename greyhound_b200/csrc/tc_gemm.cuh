@@ -48,7 +48,7 @@ constexpr int EPI_WARPS = 8;
 constexpr int EPI_CHUNKS = BN / 32 / (EPI_WARPS / 4);  // 32-column chunks per warp per half
 constexpr int TMEM_COLS = 2 * BN;
 
-enum Epi { EPI_STORE = 0, EPI_LCE = 1, EPI_LCE_Q = 2 };
+enum Epi { EPI_STORE = 0, EPI_LCE = 1, EPI_LCE_Q = 2, EPI_LSM = 3, EPI_LSM_Q = 4, EPI_LSM_GRAD = 5 };
 constexpr int kMaxPeers = 8;
 
 // Exponent window of the unnormalised-probability store (EPI_LCE_Q), in log2
@@ -60,6 +60,12 @@ constexpr int kMaxPeers = 8;
 // logsumexp is known.
 constexpr float kQHi = 80.f;
 constexpr float kQLo = -80.f;
+
+// Window of EPI_LSM_Q, narrower by 16 binary orders: there the row factor
+// g e^-lse multiplies H in 16 bits before the dW GEMM, and 2^-(64 + 17) times a
+// gradient of 2^-27 and a hidden value of 2^-7 is still a normal bf16 number.
+constexpr float kLsmQHi = 64.f;
+constexpr float kLsmQLo = -64.f;
 
 struct Params {
   int M, N, K;
@@ -88,6 +94,14 @@ struct Params {
   // EPI_LCE_Q: per (256-column tile, 128-column group, row) byte, 1 when
   // that group of the row holds raw logits instead of q ([num_n][2][M])
   uint8_t* qmode;
+  // EPI_LSM*: linear log-probabilities. Logits stay in fp32 (no rounding to
+  // the operand type) and are scaled by sc2 = log2(e) / temperature.
+  const int* tgt;         // [M] target column, negative: none
+  float sc2;
+  float* gmax;            // EPI_LSM_Q: [num_n][2][M] shift of the groups that qmode flags
+  const float* lse2;      // EPI_LSM_GRAD: [M] log-sum-exp in log2 units
+  const float* rfac;      // EPI_LSM_GRAD: [M] factor of (onehot - p)
+  const float* tval;      // EPI_LSM_GRAD: [M] value at the target column
   // EPI_STORE: optional per-row factor multiplying the product ([M] fp32)
   const float* row_scale;
   // EPI_STORE, 16-bit output: when npeer > 0 the output rows are split into
@@ -388,6 +402,18 @@ __device__ __forceinline__ void lce_fold_chunk(const uint32_t* w, int c, int n0,
   lce_target_from_chunk<OutT>(w, c, lab_rel, xt_row);
 }
 
+// One of 32 register values by a run-time index li in [0, 32), as a chain of
+// selects (an indexed load would move the array to local memory).
+__device__ __forceinline__ uint32_t select32(const uint32_t (&r)[32], int li) {
+  uint32_t v = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %2, %3;\n\tselp.b32 %0, %1, %0, p;\n\t}"
+        : "+r"(v)
+        : "r"(r[j]), "r"(li), "r"(j));
+  return v;
+}
+
 // Geometry of one configuration. PAIR = 1: one CTA computes a 128 x 256 tile.
 // PAIR = 2: a 2-CTA cluster computes a 256 x 256 tile with tcgen05.mma
 // cta_group::2; each CTA stages its 128 rows of A and 128 of the 256 B rows,
@@ -421,7 +447,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
   using G = Geo<PAIR, NSUB>;
   static_assert(NSUB == 1 || sizeof(OutT) == 2, "the 512-column tile parks 16-bit outputs only");
-  static_assert(EPI != EPI_LCE_Q || NSUB == 1, "the q store runs on 256-column tiles");
+  static_assert((EPI != EPI_LCE_Q && EPI < EPI_LSM) || NSUB == 1,
+                "the q store and the log-probability epilogues run on 256-column tiles");
   constexpr int STG = G::STG;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -860,6 +887,104 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               s_run = s_q;
             }
             if (!stats_exchange_at(h, m_run, s_run)) stop = true;
+          } else if constexpr (EPI == EPI_LSM || EPI == EPI_LSM_Q) {
+            // Log-probability statistics from the fp32 accumulator: the
+            // target's logit and, per row and 256-column tile, (max, sum of
+            // exponentials). EPI_LSM_Q also stores q = e^x in 16 bits (one
+            // ex2 does both), as e^(x - shift) with the group's largest logit
+            // as the shift where that lies outside the window: two roundings
+            // of e^x relative to itself, whatever the size of the logits.
+            // Without the store the sums are formed the same way, so that a
+            // scoring pass and a training pass over the same rows agree in
+            // every bit (the ratio of their probabilities is exactly 1).
+            const int t_rel = (row_ok ? p.tgt[row] : -1) - n0;
+            float cmax = kNegInf;
+#pragma unroll 1
+            for (int i = 0; i < EPI_CHUNKS; ++i) {
+              uint32_t r[32];
+              tc::tmem_ld32(tbase + i * 32, r);
+              tc::tmem_ld_wait(r);
+              const int col0 = n0 + (c0 + i) * 32;
+              if (col0 + 32 <= p.N) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) cmax = fmaxf(cmax, __uint_as_float(r[j]));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (col0 + j < p.N) cmax = fmaxf(cmax, __uint_as_float(r[j]));
+              }
+            }
+            const float cml = cmax * p.sc2;
+            const bool out_of_window = !(cml <= kLsmQHi && (cml >= kLsmQLo || cml == kNegInf));  // NaN: out
+            const float shift = out_of_window ? cml : 0.f;
+            float s_run = 0.f;
+            if constexpr (EPI == EPI_LSM_Q) {
+              if (row_ok && n0 + c0 * 32 < p.N) {
+                const int64_t gi = ((int64_t)nt * 2 + g) * p.M + row;
+                p.qmode[gi] = out_of_window ? 1 : 0;
+                if (out_of_window) p.gmax[gi] = cml;
+              }
+            }
+#pragma unroll 1
+            for (int i = 0; i < EPI_CHUNKS; ++i) {
+              const int c = c0 + i;
+              const int col0 = n0 + c * 32;
+              if (col0 >= p.N) break;
+              const bool full = col0 + 32 <= p.N;
+              uint32_t r[32];
+              __syncwarp();  // the target's lane may still be in its branch
+              tc::tmem_ld32(tbase + i * 32, r);
+              tc::tmem_ld_wait(r);
+              const int li = t_rel - c * 32;
+              if ((unsigned)li < 32u) p.xt[row] = __uint_as_float(select32(r, li));
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float a = fast_exp2(fmaf(__uint_as_float(r[2 * j]), p.sc2, -shift));
+                float b = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), p.sc2, -shift));
+                if (!full) {
+                  if (col0 + 2 * j >= p.N) a = 0.f;
+                  if (col0 + 2 * j + 1 >= p.N) b = 0.f;
+                }
+                s_run += a + b;
+                if constexpr (EPI == EPI_LSM_Q) w[j] = pack2<OutT>(a, b);
+              }
+              if constexpr (EPI == EPI_LSM_Q)
+                store_chunk_packed<OutT>(reinterpret_cast<OutT*>(pout), p.ldo, m0 + q * 32, p.M, col0, p.N, w,
+                                         stage_out, lane, p.vec_ok, p.out_evict_first);
+            }
+            const float m_run = s_run == 0.f ? kNegInf : shift;  // a NaN sum must not look empty to the merge
+            __syncwarp();
+            if (!stats_exchange_at(h, m_run, s_run)) stop = true;
+          } else if constexpr (EPI == EPI_LSM_GRAD) {
+            // The logits' gradient straight from the recomputed accumulator:
+            // rfac (onehot - e^(x - lse)), rounded once. The target's own value
+            // comes from -expm1(log-probability): no cancellation at p near 1.
+            const int t = row_ok ? p.tgt[row] : -1;
+            const float l2 = row_ok && t >= 0 ? p.lse2[row] : 0.f;
+            const float f = row_ok && t >= 0 ? p.rfac[row] : 0.f;
+            const uint32_t tv = __float_as_uint(row_ok && t >= 0 ? p.tval[row] : 0.f);
+#pragma unroll 1
+            for (int i = 0; i < EPI_CHUNKS; ++i) {
+              const int c = c0 + i;
+              const int col0 = n0 + c * 32;
+              if (col0 >= p.N) break;
+              uint32_t r[32];
+              tc::tmem_ld32(tbase + i * 32, r);
+              tc::tmem_ld_wait(r);
+              const int li = t - col0;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float d = -f * fast_exp2(fmaf(__uint_as_float(r[j]), p.sc2, -l2));
+                r[j] = t < 0 ? 0u : li == j ? tv : __float_as_uint(d);  // a row without a target: 0 even where NaN
+              }
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                w[j] = pack2<OutT>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+              store_chunk_packed<OutT>(reinterpret_cast<OutT*>(pout), p.ldo, m0 + q * 32, p.M, col0, p.N, w,
+                                       stage_out, lane, p.vec_ok, p.out_evict_first);
+            }
           } else if constexpr (EPI == EPI_LCE) {
             const int64_t lab = row_ok ? p.labels[row] - p.label_offset : -1;
             const int64_t lab_rel = lab - n0;  // label column inside this half, if any

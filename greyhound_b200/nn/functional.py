@@ -2,7 +2,8 @@
 
 ``selective_log_softmax`` (:53-69), ``cross_entropy`` (:72-116),
 ``autograd_loss_and_logits_grad`` (:119-148), ``chunked_linear_loss`` (:151-223)
-and ``chunked_linear_cross_entropy`` (:226-287). ``weight`` is ``[V, D]`` and is
+and ``chunked_linear_cross_entropy`` (:226-287).
+``chunked_linear_selective_log_softmax`` has no counterpart there. ``weight`` is ``[V, D]`` and is
 handed to the ops as the ``[D, V]`` view ``weight.T``, exactly as the reference
 does, so the op schemas and their fakes are unchanged.
 """
@@ -17,6 +18,7 @@ from torch import Tensor
 
 from greyhound_b200.ops.chunked_linear_cross_entropy import ChunkedLinearCrossEntropyFunction
 from greyhound_b200.ops.chunked_linear_loss import ChunkedLinearLossFunction
+from greyhound_b200.ops.chunked_linear_selective_log_softmax import ChunkedLinearSelectiveLogSoftmaxFunction
 from greyhound_b200.ops.cross_entropy import CrossEntropyFunction
 from greyhound_b200.ops.logprobs import SelectiveLogSoftmaxFunction
 
@@ -26,6 +28,7 @@ __all__ = [
     "autograd_loss_and_logits_grad",
     "chunked_linear_loss",
     "chunked_linear_cross_entropy",
+    "chunked_linear_selective_log_softmax",
 ]
 
 
@@ -159,3 +162,47 @@ def chunked_linear_cross_entropy(
             grad_weight_accum_dtype == "fp32",
         ),
     )
+
+
+def chunked_linear_selective_log_softmax(
+    inputs: Tensor,
+    weight: Tensor,
+    index: Tensor,
+    ignore_index: int = -100,
+    temperature: float = 1.0,
+    grad_weight_accum_dtype: Literal["fp32", "weight"] = "fp32",
+) -> Tensor:
+    """Log-probability of ``index`` under ``softmax(inputs @ weight.T / temperature)``.
+
+    ``selective_log_softmax`` from hidden states, without the logits:
+    ``inputs`` is ``[..., D]`` and ``weight`` ``[V, D]``, both bf16 or both
+    fp16, with ``D`` a multiple of 8; ``index`` has ``inputs``' leading shape,
+    int32 or int64. The result has ``index``'s shape and is fp32, computed from
+    unrounded fp32 logits (ratios of probabilities need more than 16 bits).
+
+    Positions where ``index == ignore_index`` give 0 and no gradient, whatever
+    their hidden state holds. An index outside ``[0, V)`` gives NaN and no
+    gradient, and the next call on the device raises ``ValueError``.
+
+    Differentiable (once) with respect to ``inputs`` and ``weight``, for any
+    gradient of the log-probabilities. bf16 operands with ``N * V * 2`` bytes
+    up to 4 GiB keep ``e^x`` from the forward for that; otherwise the backward
+    recomputes the logits in row chunks, summing the weight gradient over the
+    chunks in fp32 or, with ``grad_weight_accum_dtype="weight"``, in the
+    parameter's type.
+    """
+    _check_accum_dtype(grad_weight_accum_dtype)
+    if inputs.ndim < 1 or index.shape != inputs.shape[:-1]:
+        raise ValueError(f"expected index shape {tuple(inputs.shape[:-1])}, got {tuple(index.shape)}")
+    flat = cast(
+        Tensor,
+        ChunkedLinearSelectiveLogSoftmaxFunction.apply(
+            inputs.reshape(-1, inputs.shape[-1]) if inputs.shape[-1] else inputs.reshape(index.numel(), 0),
+            weight,
+            index.reshape(-1),
+            ignore_index,
+            float(temperature),
+            grad_weight_accum_dtype == "fp32",
+        ),
+    )
+    return flat.reshape(index.shape)

@@ -326,6 +326,42 @@ GH_API int gh_gemm(const void* A, int64_t lda, int a_mn_major,
  * ------------------------------------------------------------------------ */
 GH_API int gh_scale(const void* in, void* out, int64_t n, int dtype, const float* g, void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Linear selective log-softmax (no counterpart in the reference, whose
+ * log-probabilities start from logits, kernels/logprobs.py:131):
+ *   x = H W^T * inv_temperature; logprobs[r] = x[r, index[r]] - logsumexp(x[r])
+ * in fp32 from the fp32 accumulator, without the [N, V] logits in memory.
+ *   H [N, D], W [V, D] in {F16, BF16}, D % 8 == 0, 16-byte aligned
+ *   index [N] in {I32, I64}: rows equal to ignore_index give 0 and no
+ *           gradient; an index outside [0, V) gives NaN, no gradient, and
+ *           GH_DEV_BAD_LABEL
+ *   lse2    [N] log-sum-exp in log2 units (optional; gh_lsm_bwd needs it)
+ *   kept    optional (BF16), gh_lsm_kept_bytes(): e^x in 16 bits and the row
+ *           factors, which gh_lsm_bwd_kept reads (any number of times)
+ * The backward takes the gradient `grad` [N] (F32) of logprobs and writes
+ * grad_input [N, D] and / or grad_weight [V, D] (NULL: not computed) in the
+ * operand type: gh_lsm_bwd_kept with two GEMMs, gh_lsm_bwd by repeating the
+ * logits GEMM chunk_rows rows at a time, summing grad_weight over the chunks
+ * in fp32 or (fp32_grad_weight_accum = 0) in the operand type.
+ * ------------------------------------------------------------------------ */
+GH_API size_t gh_lsm_kept_bytes(int64_t N, int64_t V);
+GH_API size_t gh_lsm_fwd_workspace_bytes(int64_t N, int64_t V, int64_t chunk_rows, int keep);
+GH_API size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t chunk_rows, int kept,
+                                         int fp32_grad_weight_accum);
+GH_API int gh_lsm_fwd(const void* H, const void* W, const void* index, int index_dtype, int64_t N, int64_t D,
+                      int64_t V, int dtype, int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
+                      float* logprobs, float* lse2, void* kept, size_t kept_bytes, void* workspace,
+                      size_t workspace_bytes, void* stream);
+GH_API int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V,
+                           int dtype, double inv_temperature, const void* kept, size_t kept_bytes,
+                           void* grad_input, void* grad_weight, void* workspace, size_t workspace_bytes,
+                           void* stream);
+GH_API int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* logprobs,
+                      const float* lse2, const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
+                      int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
+                      int fp32_grad_weight_accum, void* grad_input, void* grad_weight, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* Optional event timing of the library's launches, by kernel class:
  * 0 logits GEMM + fused CE epilogue, 1 dW GEMM, 2 dH GEMM, 3 dlogits pass,
  * 4 standalone row kernels, 5 other GEMMs. gh_profile_read synchronises on

@@ -1,0 +1,68 @@
+"""chunked_linear_selective_log_softmax refuses what it cannot take, before any
+device call; the buffer sizes of its passes."""
+
+import pytest
+import torch
+
+from greyhound_b200 import _lib
+from greyhound_b200.nn.functional import chunked_linear_selective_log_softmax as f
+
+BF = torch.bfloat16
+
+
+def z(*s, dtype=BF):
+    return torch.zeros(*s, dtype=dtype)
+
+
+@pytest.mark.parametrize(
+    "args,kw,error,match",
+    [
+        ((z(4, 16), z(9, 16), z(4, dtype=torch.int64)), {}, ValueError, "same CUDA device"),
+        ((z(4, 16), z(9, 24), z(4, dtype=torch.int64)), {}, ValueError, "expected inputs"),
+        ((z(4, 16), z(16), z(4, dtype=torch.int64)), {}, ValueError, "expected inputs"),
+        ((z(4, 16), z(9, 16), z(5, dtype=torch.int64)), {}, ValueError, "index shape"),
+        ((z(4, 16), z(9, 16), z(4, 1, dtype=torch.int64)), {}, ValueError, "index shape"),
+        ((z(4, 16, dtype=torch.float32), z(9, 16, dtype=torch.float32), z(4, dtype=torch.int64)), {}, TypeError, "float16 or bfloat16"),
+        ((z(4, 16), z(9, 16, dtype=torch.float16), z(4, dtype=torch.int64)), {}, TypeError, "weight of dtype"),
+        ((z(4, 16), z(9, 16), z(4, dtype=torch.int16)), {}, TypeError, "int32 or int64"),
+        ((z(4, 12), z(9, 12), z(4, dtype=torch.int64)), {}, ValueError, "multiple of 8"),
+        ((z(4, 0), z(9, 0), z(4, dtype=torch.int64)), {}, ValueError, "multiple of 8"),
+        ((z(4, 16), z(0, 16), z(4, dtype=torch.int64)), {}, ValueError, "non-empty vocabulary"),
+        ((z(4, 16), z(9, 16), z(4, dtype=torch.int64)), {"temperature": 0.0}, ValueError, "temperature"),
+        ((z(4, 16), z(9, 16), z(4, dtype=torch.int64)), {"temperature": float("nan")}, ValueError, "temperature"),
+        ((z(4, 16), z(9, 16), z(4, dtype=torch.int64)), {"temperature": float("inf")}, ValueError, "temperature"),
+        ((z(4, 16), z(9, 16), z(4, dtype=torch.int64)), {"grad_weight_accum_dtype": "bf16"}, ValueError, "grad_weight_accum"),
+    ],
+)
+def test_refusals(args, kw, error, match):
+    with pytest.raises(error, match=match):
+        f(*args, **kw)
+
+
+def test_c_entries_refuse_bad_arguments():
+    lib = _lib.load()
+    fwd = lambda dtype=_lib.GH_BF16, D=16, kept=None, kb=0, wb=1 << 30, inv_t=1.0, idt=_lib.GH_I64: lib.gh_lsm_fwd(  # noqa: E731
+        8, 8, 8, idt, 4, D, 9, dtype, -100, inv_t, 4, 8, 8, kept, kb, 8, wb, None)
+    for st, error in (
+        (fwd(dtype=_lib.GH_F32), TypeError),
+        (fwd(idt=_lib.GH_F32), TypeError),
+        (fwd(D=12), ValueError),
+        (fwd(inv_t=0.0), ValueError),
+        (fwd(wb=16), RuntimeError),
+        (fwd(kept=8, kb=16), RuntimeError),
+        (fwd(dtype=_lib.GH_F16, kept=8, kb=1 << 20), RuntimeError),
+        (lib.gh_lsm_bwd_kept(8, 8, 8, 4, 16, 9, _lib.GH_F16, 1.0, 8, 1 << 20, 8, 8, 8, 1 << 30, None), RuntimeError),
+        (lib.gh_lsm_bwd_kept(8, 8, 8, 4, 16, 9, _lib.GH_BF16, 1.0, 8, 1 << 20, 8, 8, 8, 16, None), RuntimeError),
+        (lib.gh_lsm_bwd(8, 8, None, _lib.GH_I64, 8, 8, 8, 4, 16, 9, _lib.GH_BF16, -100, 1.0, 4, 1, 8, 8, 8, 1 << 30, None), ValueError),
+    ):
+        with pytest.raises(error):
+            _lib.check(st, "x")
+
+
+def test_buffer_sizes():
+    """Stored e^x is 2 bytes a logit; the forward without it, and the
+    recomputed backward, do not grow with N * V."""
+    lib = _lib.load()
+    assert lib.gh_lsm_kept_bytes(8192, 128256) < 8192 * 128256 * 2 + (1 << 20)
+    assert lib.gh_lsm_fwd_workspace_bytes(65536, 128256, 8192, 0) < 64 << 20
+    assert lib.gh_lsm_bwd_workspace_bytes(65536, 4096, 128256, 8192, 0, 1) < (2 << 30) + 4 * 4096 * 128256 + (256 << 20)

@@ -1,0 +1,313 @@
+"""chunked_linear_selective_log_softmax against its definition in 64 bits.
+
+Tolerances (u = 2^-8 for bf16, 2^-11 for fp16, relative):
+ * log-probabilities: fp32 logits with the tensor core's accumulation. Each of
+   the D / 16 steps may lose up to 2^-23 of the running sum, which is at most
+   S = max_v sum_d |H W| / temperature; the target's logit and the log-sum-exp
+   each carry that, so |error| <= 2 (D / 16 + 4) 2^-23 S + 2^-20 (exponentials).
+ * gradients: each product of a sum carries one rounding of the logits'
+   gradient or of e^x (u), in the kept form another of the row (u) and of
+   the target's share (u), and the result one of its own (u), or two where
+   split-K adds 16-bit halves (2 u). So |error| <= 3 u sum |terms| + 2 u |result|
+   plus, where a log-probability is off by e, e p |g| in its term (a
+   probability moves by e p, and so does 1 - p at the target).
+ * underflow: e^x below 2^-126 counts as 0 (ex2.ftz), and a row stored as e^x
+   has a log-sum-exp of at least 2^-64, so a probability may be off by
+   2^-126 / 2^-64 = 2^-62 absolutely: 2^-62 |g| sum |H| (or |W|) in the gradients.
+"""
+
+import math
+
+import pytest
+import torch
+from torch.library import opcheck
+
+from greyhound_b200.kernels import linear_logprobs as K
+from greyhound_b200.nn.functional import chunked_linear_selective_log_softmax
+from greyhound_b200.ops.chunked_linear_selective_log_softmax import (
+    linear_selective_log_softmax,
+    linear_selective_log_softmax_bwd,
+    linear_selective_log_softmax_kept,
+    linear_selective_log_softmax_kept_bwd,
+)
+from greyhound_b200.testing import requires_gpu
+
+U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+
+
+def make(N, D, V, dtype, seed, scale=1.0, left_out=0.1, index_dtype=torch.int64):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    H = torch.randn(N, D, device="cuda", generator=g).to(dtype)
+    W = (torch.randn(V, D, device="cuda", generator=g) * (scale / math.sqrt(D))).to(dtype)
+    t = torch.randint(0, V, (N,), device="cuda", generator=g).to(index_dtype)
+    if N > 1:
+        t[torch.rand(N, device="cuda", generator=g) < left_out] = -100
+    return H, W, t, torch.randn(N, device="cuda", generator=g)
+
+
+def definition(H, W, t, g, temperature=1.0):
+    """(logprobs, dH, dW, bounds of the three) in 64 bits."""
+    u = U[H.dtype]
+    H, W = H.double(), W.double()
+    x = H @ W.T / temperature
+    lp = torch.log_softmax(x, 1)
+    on = t != -100
+    at = t.long().clamp(min=0)[:, None]
+    y = torch.where(on, lp.gather(1, at)[:, 0], 0.0)
+    g = (torch.where(on, g.double(), 0.0) / temperature)[:, None]
+    d = torch.zeros_like(x).scatter_(1, at, g) - g * lp.exp()
+    S = (H.abs() @ W.abs().T / temperature).amax()
+    ey = 2 * (H.shape[1] / 16 + 4) * 2.0**-23 * S + 2.0**-20
+    dH, dW = d @ W, d.T @ H
+    a = 3 * u * d.abs() + ey * g.abs() * lp.exp()
+    bH = a @ W.abs() + 2 * u * dH.abs() + 2.0**-62 * g.abs() * W.abs().sum(0)
+    bW = a.T @ H.abs() + 2 * u * dW.abs() + 2.0**-62 * (g.abs() * H.abs()).sum(0)
+    tiny = 2.0**-24 if u == 2.0**-11 else 0.0  # fp16's spacing near zero, of the results
+    return y, dH, dW, ey, bH + tiny, bW + tiny
+
+
+def check(H, W, t, g, temperature=1.0, **kw):
+    h, w = H.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, w, t, temperature=temperature, **kw)
+    dh, dw = torch.autograd.grad(y, (h, w), g)
+    ry, rH, rW, ey, bH, bW = definition(H, W, t, g, temperature)
+    assert y.dtype == torch.float32 and y.shape == t.shape
+    assert dh.dtype == H.dtype and dw.dtype == W.dtype
+    assert ((y.double() - ry).abs() <= ey).all(), ((y.double() - ry).abs().max(), ey)
+    assert ((dh.double() - rH).abs() <= bH).all(), ((dh.double() - rH).abs() / bH).max()
+    assert ((dw.double() - rW).abs() <= bW).all(), ((dw.double() - rW).abs() / bW).max()
+    skip = t == -100
+    assert (y[skip] == 0).all() and (dh[skip] == 0).all()
+    return y, dh, dw
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize(
+    "N,D,V",
+    [(1, 8, 1), (1, 64, 300), (3, 8, 7), (2, 72, 257), (127, 64, 255), (128, 136, 256), (129, 128, 513), (300, 264, 1000),
+     (513, 512, 4099), (1030, 320, 2051)],
+)
+def test_against_definition(N, D, V, dtype):
+    check(*make(N, D, V, dtype, N + D + V, scale=2.0))
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("temperature", [0.3, 1.7])
+def test_temperature(dtype, temperature):
+    check(*make(200, 128, 3001, dtype, 5, scale=1.5), temperature=temperature)
+
+
+@requires_gpu
+@pytest.mark.parametrize("accum", ["fp32", "weight"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_recomputed_backward_over_several_chunks(monkeypatch, dtype, accum):
+    """Chunks of 128 rows, the last one short: with fp32 accumulation the same
+    bound; in the operand type each of the 4 partial sums is rounded (u each,
+    relative to a partial sum of at most the sum of absolute terms)."""
+    monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    monkeypatch.setattr(K, "_chunk", lambda N, D, V: 128)
+    H, W, t, g = make(400, 128, 1111, dtype, 9, scale=2.0)
+    if accum == "fp32":
+        check(H, W, t, g)
+        return
+    h, w = H.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, w, t, grad_weight_accum_dtype=accum)
+    _, dw = torch.autograd.grad(y, (h, w), g)
+    _, _, rW, _, _, bW = definition(H, W, t, g)
+    assert ((dw.double() - rW).abs() <= bW * (7 / 3)).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("scale", [30.0, 120.0])
+def test_logits_outside_the_exponent_window(scale):
+    """Largest logits of about 100 and 400 (the stored e^x covers +-44): rows
+    are rewritten, with the same bound; p_t near 1 and near 0 both occur."""
+    H, W, t, g = make(160, 64, 900, torch.bfloat16, 3, scale=scale)
+    t[::2] = (H[::2].double() @ W.double().T).argmax(1)
+    check(H, W, t, g)
+
+
+@requires_gpu
+def test_rows_of_very_small_and_shifted_logits():
+    """Every logit of a row near -400 (below the window), beside normal rows."""
+    H, W, t, g = make(130, 64, 700, torch.bfloat16, 4)
+    W[:, 0] = 20.0
+    H[:, 0] = 0.0
+    H[::3, 0] = -20.0
+    H[1::3, 0] = 20.0
+    check(H, W, t, g)
+
+
+@requires_gpu
+def test_confident_targets_keep_their_gradient():
+    """1 - p_t far below one 16-bit step of p_t."""
+    H, W, t, g = make(64, 64, 500, torch.bfloat16, 6, left_out=0.0)
+    H[:, 0] = 4.0
+    W[:, 0] = 0.0
+    W[17, 0] = 4.0
+    t[:] = 17
+    y, dh, _ = check(H, W, t, g)
+    assert (y < 0).all() and (dh != 0).any(1).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("kept", [True, False])
+def test_left_out_rows_may_hold_anything(monkeypatch, kept):
+    if not kept:
+        monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    H, W, t, g = make(200, 64, 300, torch.bfloat16, 8)
+    t[5], t[77], t[199] = -100, -100, -100
+    clean = check(H, W, t, g)
+    H[5], H[77, 3], H[199] = float("nan"), float("inf"), 3e38
+    g[5], g[77] = float("nan"), float("inf")
+    h, w = H.requires_grad_(True), W.requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, w, t)
+    dh, dw = torch.autograd.grad(y, (h, w), g)
+    assert torch.equal(y.detach(), clean[0].detach()) and torch.equal(dh, clean[1]) and torch.equal(dw, clean[2])
+
+
+@requires_gpu
+def test_nan_rows_stay_their_own():
+    H, W, t, g = make(70, 64, 300, torch.bfloat16, 8, left_out=0.0)
+    clean = check(H, W, t, g)
+    H[9, 1] = float("nan")
+    h = H.requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, W, t)
+    (dh,) = torch.autograd.grad(y, h, g)
+    rest = torch.arange(70, device="cuda") != 9
+    assert y[9].isnan() and dh[9].isnan().all()
+    assert torch.equal(y[rest], clean[0][rest]) and torch.equal(dh[rest], clean[1][rest])
+
+
+@requires_gpu
+def test_one_gradient_alone_and_no_gradient():
+    H, W, t, g = make(150, 128, 1000, torch.bfloat16, 11)
+    y, dh, dw = check(H, W, t, g)
+    assert torch.equal(chunked_linear_selective_log_softmax(H, W, t), y.detach())
+    for keep in (K._KEEP_BYTES, 0):
+        K._KEEP_BYTES, before = keep, K._KEEP_BYTES
+        try:
+            h = H.clone().requires_grad_(True)
+            (a,) = torch.autograd.grad(chunked_linear_selective_log_softmax(h, W, t), h, g)
+            w = W.clone().requires_grad_(True)
+            (b,) = torch.autograd.grad(chunked_linear_selective_log_softmax(H, w, t), w, g)
+        finally:
+            K._KEEP_BYTES = before
+        if keep:
+            assert torch.equal(a, dh) and torch.equal(b, dw)
+
+
+@requires_gpu
+@pytest.mark.parametrize("scale", [1.0, 100.0])
+def test_scoring_and_training_forwards_agree_in_every_bit(monkeypatch, scale):
+    """The policy's ratio against log-probabilities taken without a gradient is exactly 1."""
+    H, W, t, g = make(300, 192, 1500, torch.bfloat16, 21, scale=scale)
+    scored = chunked_linear_selective_log_softmax(H, W, t)
+    h = H.clone().requires_grad_(True)
+    assert torch.equal(chunked_linear_selective_log_softmax(h, W, t).detach(), scored)
+    monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    assert torch.equal(chunked_linear_selective_log_softmax(h, W, t).detach(), scored)
+
+
+@requires_gpu
+def test_retained_graph_takes_other_gradients():
+    H, W, t, g = make(150, 128, 1000, torch.bfloat16, 12)
+    h, w = H.requires_grad_(True), W.requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, w, t)
+    first = torch.autograd.grad(y, (h, w), g, retain_graph=True)
+    torch.autograd.grad(y, (h, w), -3 * g, retain_graph=True)
+    again = torch.autograd.grad(y, (h, w), g)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@requires_gpu
+def test_layouts():
+    """Leading dimensions, int32 indices, strided and misaligned operands, an expanded gradient."""
+    H, W, t, g = make(120, 64, 333, torch.bfloat16, 13)
+    y, dh, dw = check(H, W, t, g)
+    y3 = chunked_linear_selective_log_softmax(H.view(4, 30, 64), W, t.view(4, 30).int())
+    assert y3.shape == (4, 30) and torch.equal(y3.view(-1), y.detach())
+    odd = torch.empty(120 * 64 + 1, dtype=H.dtype, device="cuda")[1:].view(120, 64).copy_(H)
+    assert odd.data_ptr() % 16
+    wide = torch.empty(333, 128, dtype=W.dtype, device="cuda")[:, ::2].copy_(W)
+    assert torch.equal(chunked_linear_selective_log_softmax(odd, wide, t), y.detach())
+    h = H.clone().requires_grad_(True)
+    chunked_linear_selective_log_softmax(h, W, t).sum().backward()
+    ones = torch.autograd.grad(chunked_linear_selective_log_softmax(h, W, t), h, torch.ones(120, device="cuda"))[0]
+    assert torch.equal(h.grad, ones)
+
+
+@requires_gpu
+def test_no_rows():
+    H = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    W = torch.randn(100, 64, device="cuda").bfloat16().requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(H, W, torch.empty(0, device="cuda", dtype=torch.int64))
+    dh, dw = torch.autograd.grad(y.sum(), (H, W))
+    assert y.shape == (0,) and dh.shape == (0, 64) and (dw == 0).all()
+
+
+@requires_gpu
+def test_bad_index_is_reported_and_harmless():
+    H, W, t, g = make(64, 64, 100, torch.bfloat16, 14, left_out=0.0)
+    t[3], t[4] = 100, -7
+    y = chunked_linear_selective_log_softmax(H, W, t)
+    torch.cuda.synchronize()
+    assert y[3].isnan() and y[4].isnan() and torch.isfinite(y[5:]).all()
+    with pytest.raises(ValueError, match="outside"):
+        chunked_linear_selective_log_softmax(H, W, t.clamp(0, 99))
+
+
+@requires_gpu
+def test_against_differences():
+    """Directional derivative of the definition, in 64 bits, at two points around H."""
+    H, W, t, g = make(48, 64, 200, torch.float16, 15)
+    _, dh, _ = check(H, W, t, g)
+    v = torch.randn(48, 64, device="cuda", dtype=torch.float64)
+    e = 1e-4
+
+    def f(h):
+        lp = torch.log_softmax(h @ W.double().T, 1).gather(1, t.clamp(min=0)[:, None])[:, 0]
+        return (torch.where(t != -100, lp, 0.0) * g.double()).sum()
+
+    numeric = (f(H.double() + e * v) - f(H.double() - e * v)) / (2 * e)
+    # second-order rest of the difference, and the kernel's own bound over the direction
+    _, _, _, _, bH, _ = definition(H, W, t, g)
+    assert (numeric - (dh.double() * v).sum()).abs() <= (bH * v.abs()).sum() + 1e-4
+
+
+@requires_gpu
+def test_opcheck():
+    H, W, t, g = make(40, 64, 130, torch.bfloat16, 16)
+    opcheck(linear_selective_log_softmax, (H, W, t, -100, 1.0))
+    opcheck(linear_selective_log_softmax_kept, (H, W, t, -100, 1.0), test_utils=["test_schema", "test_faketensor"])
+    y, lse2 = linear_selective_log_softmax(H, W, t, -100, 1.0)
+    opcheck(linear_selective_log_softmax_bwd, (H, W, t, y, lse2, g, -100, 1.0, True, True, False))
+    _, kept = linear_selective_log_softmax_kept(H, W, t, -100, 1.0)
+    opcheck(linear_selective_log_softmax_kept_bwd, (H, W, kept, g, 1.0, True, True))
+
+
+@requires_gpu
+def test_deterministic_and_capturable():
+    H, W, t, g = make(300, 128, 2000, torch.bfloat16, 17)
+    h, w = H.requires_grad_(True), W.requires_grad_(True)
+
+    def step():
+        y = chunked_linear_selective_log_softmax(h, w, t)
+        return y, *torch.autograd.grad(y, (h, w), g)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            eager = [a.detach().clone() for a in step()]
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, eager):
+        assert torch.equal(a.detach(), b)
