@@ -22,6 +22,8 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgreyhound_b200.so"
 GH_F16, GH_BF16, GH_F32, GH_I32, GH_I64 = 0, 1, 2, 3, 4
 GH_OK, GH_EINVAL, GH_ETYPE, GH_ECUDA, GH_EWORKSPACE, GH_EUNSUPPORTED = 0, 1, 2, 3, 4, 5
 GH_DEV_BAD_LABEL = 1
+GH_DEV_BAD_SEQLENS = 2
+GH_DEV_AMBIGUOUS = 8
 GH_DEV_PIPELINE_TIMEOUT = 4
 
 DTYPE_CODE = {
@@ -107,6 +109,22 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i64, _f64, _i64, _i32, _vp, _vp, _vp, _sz,
          _vp],
     ),
+    "gh_policy_loss_workspace_bytes": (_sz, [_i64, _i64, _i32]),
+    "gh_policy_loss_fwd": (
+        _i32,
+        [_vp, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _vp, _i32, _i64, _f64, _f64, _f64, _i32, _vp, _vp, _vp,
+         _vp, _vp, _sz, _vp],
+    ),
+    "gh_policy_loss_bwd": (_i32, [_vp, _vp, _vp, _sz, _vp, _i64, _vp, _i32, _i64, _i32, _vp, _i32, _vp]),
+    "gh_preference_loss_workspace_bytes": (_sz, [_i64, _i64]),
+    "gh_preference_loss_fwd": (
+        _i32,
+        [_vp, _i32, _vp, _i32, _vp, _i64, _vp, _i32, _i64, _f64, _f64, _f64, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
+         _sz, _vp],
+    ),
+    "gh_preference_loss_bwd": (_i32, [_vp, _vp, _vp, _i64, _vp, _i32, _i64, _vp, _i32, _vp]),
+    "gh_global_norm_workspace_bytes": (_sz, [_i64]),
+    "gh_clip_by_global_norm": (_i32, [_vp, _vp, _vp, _vp, _i64, _f64, _i32, _vp, _vp, _sz, _vp]),
     "gh_profile_enable": (None, [_i32]),
     "gh_profile_read": (_i32, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_longlong), _i32, _i32]),
 }
@@ -240,6 +258,13 @@ def _raise_bits(bits: int, what: str) -> None:
     if bits & GH_DEV_BAD_LABEL:
         raise ValueError(f"{what}: a target / index outside [0, vocab) that is not ignore_index "
                          "(recorded on the device by an earlier greyhound_b200 call)")
+    if bits & GH_DEV_BAD_SEQLENS:
+        raise ValueError(f"{what}: sequence offsets (cu_seqlens) that decrease or leave [0, tokens] "
+                         "(recorded on the device by an earlier greyhound_b200 call)")
+    if bits & GH_DEV_AMBIGUOUS:
+        raise ValueError(f"{what}: as many packed advantages as tokens and as sequences, which do not hold one "
+                         "token each; say advantages_per=\"token\" or \"sequence\" (recorded on the device by an "
+                         "earlier greyhound_b200 call)")
     if bits:
         raise GreyhoundLibraryError(f"{what}: device status {bits:#x} (a GEMM pipeline wait timed out "
                                     "in an earlier greyhound_b200 call; its results are not valid)")
@@ -267,3 +292,12 @@ def raise_on_status(ws: torch.Tensor, what: str) -> None:
     st = device_status(ws)
     take_device_errors(ws.device)  # reported here; do not report it twice
     _raise_bits(st, what)
+
+
+def raise_on_report(device: torch.device, what: str) -> None:
+    """``raise_on_status`` for calls without a status word, whose kernels
+    report to the device's sticky slot themselves."""
+    if not CHECK_STATUS:
+        return
+    torch.cuda.current_stream(device).synchronize()
+    raise_pending(device, what)

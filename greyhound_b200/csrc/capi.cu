@@ -63,8 +63,7 @@ int* error_slots() {
   return g_slots;
 }
 
-int publish_status(const int* status, cudaStream_t st) {
-  if (!status) return GH_OK;
+int device_error_slot(int** slot) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_error(GH_ECUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
@@ -74,7 +73,16 @@ int publish_status(const int* status, cudaStream_t st) {
   void* dslot = nullptr;
   e = cudaHostGetDevicePointer(&dslot, slots + dev, 0);
   if (e != cudaSuccess) return set_error(GH_ECUDA, "cudaHostGetDevicePointer: %s", cudaGetErrorString(e));
-  publish_status_kernel<<<1, 1, 0, st>>>(status, static_cast<int*>(dslot));
+  *slot = static_cast<int*>(dslot);
+  return GH_OK;
+}
+
+int publish_status(const int* status, cudaStream_t st) {
+  if (!status) return GH_OK;
+  int* dslot = nullptr;
+  const int rc = device_error_slot(&dslot);
+  if (rc) return rc;
+  publish_status_kernel<<<1, 1, 0, st>>>(status, dslot);
   count_launch(1);
   return check_launch("publish_status");
 }

@@ -27,6 +27,9 @@ void count_launch(int n = 1);
 // Enqueue the copy of a non-zero workspace status word into this device's
 // sticky error slot (gh_take_device_errors); GH_OK when status is NULL.
 int publish_status(const int* status, cudaStream_t st);
+// Device address of the current device's sticky error slot, for a kernel that
+// reports a problem there itself.
+int device_error_slot(int** slot);
 
 // Kernel classes for the optional event timing (gh_profile_enable / _read).
 enum ProfClass {
@@ -128,6 +131,15 @@ __device__ __forceinline__ U8 ld32_keep(const void* p) {
 __device__ __forceinline__ U8 ld32_last(const void* p) {
   U8 v;
   asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]),
+                 "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p));
+  return v;
+}
+// The same for memory that this kernel writes, too: not the read-only path.
+__device__ __forceinline__ U8 ld32_last_rw(const void* p) {
+  U8 v;
+  asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]),
                  "=r"(v.w[6]), "=r"(v.w[7])
                : "l"(p));

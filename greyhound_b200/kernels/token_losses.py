@@ -1,0 +1,281 @@
+"""Losses over per-token log-probabilities (sm_100a, via the C-ABI): the clipped
+policy loss with a KL term, and the preference loss over pairs of sequences.
+
+Log-probabilities are padded ``[sequences, length]`` or packed ``[tokens]`` with
+offsets ``cu_seqlens``; a boolean mask may leave positions out.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from greyhound_b200 import _lib
+
+__all__ = [
+    "policy_loss_forward",
+    "policy_loss_backward",
+    "preference_loss_forward",
+    "preference_loss_backward",
+    "policy_workspace_bytes",
+]
+
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+REDUCTIONS = {"sum": 0, "mean": 1, "sequence_mean": 2}
+KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+ADVANTAGES_PER = {"token": 0, "sequence": 1, "auto": 2}
+
+
+class _Layout(NamedTuple):
+    tokens: int
+    seqs: int
+    cu: Tensor | None
+    cu_code: int
+
+
+def _check_like(name: str, t: Tensor, logprobs: Tensor) -> None:
+    if t.shape != logprobs.shape:
+        raise ValueError(f"expected {name} shape {tuple(logprobs.shape)}, got {tuple(t.shape)}")
+    if t.device != logprobs.device:
+        raise ValueError(f"expected {name} on {logprobs.device}, got {t.device}")
+
+
+def _no_grad_to(**tensors: Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f"the loss is not differentiable with respect to {name}; pass {name}.detach()")
+
+
+def _layout(logprobs: Tensor, mask: Tensor | None, cu_seqlens: Tensor | None) -> _Layout:
+    if logprobs.ndim not in (1, 2):
+        raise ValueError(f"expected logprobs [sequences, length] or [tokens], got shape {tuple(logprobs.shape)}")
+    if logprobs.dtype not in _FLOATS:
+        raise TypeError(f"unsupported logprobs dtype: {logprobs.dtype}")
+    if mask is not None:
+        _check_like("mask", mask, logprobs)
+        if mask.dtype != torch.bool:
+            raise TypeError(f"expected a bool mask, got {mask.dtype}")
+    if cu_seqlens is not None:
+        if logprobs.ndim != 1:
+            raise ValueError("cu_seqlens goes with packed logprobs [tokens]")
+        if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
+            raise ValueError(f"expected cu_seqlens [sequences + 1], got shape {tuple(cu_seqlens.shape)}")
+        if cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"expected int32 or int64 cu_seqlens, got {cu_seqlens.dtype}")
+        if cu_seqlens.device != logprobs.device:
+            raise ValueError(f"expected cu_seqlens on {logprobs.device}, got {cu_seqlens.device}")
+    if not logprobs.is_cuda:
+        raise ValueError("expected logprobs on a CUDA device (greyhound_b200 has no CPU path)")
+    if cu_seqlens is not None:
+        return _Layout(logprobs.numel(), cu_seqlens.numel() - 1, cu_seqlens.contiguous(),
+                       _lib.dtype_code(cu_seqlens.dtype))
+    return _Layout(logprobs.numel(), logprobs.shape[0] if logprobs.ndim == 2 else 1, None, 0)
+
+
+def _others(logprobs: Tensor, *ts: Tensor | None) -> tuple[int, list[Tensor | None]]:
+    """The other log-probabilities, all in logprobs' type or all in fp32."""
+    for t in ts:
+        if t is not None and not t.is_floating_point():
+            raise TypeError(f"unsupported log-probability dtype: {t.dtype}")
+    same = all(t is None or t.dtype == logprobs.dtype for t in ts)
+    dtype = logprobs.dtype if same else torch.float32
+    return _lib.dtype_code(dtype), [None if t is None else t.to(dtype).contiguous() for t in ts]
+
+
+def policy_workspace_bytes(logprobs: Tensor, cu_seqlens: Tensor | None, reduction: str) -> int:
+    seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None else logprobs.shape[0] if logprobs.ndim == 2 else 1
+    return max(int(_lib.load().gh_policy_loss_workspace_bytes(logprobs.numel(), seqs, REDUCTIONS[reduction])), 256)
+
+
+def _advantages(advantages: Tensor, logprobs: Tensor, lay: _Layout, per: str) -> tuple[Tensor, int]:
+    """(contiguous fp32 advantages, the C-ABI's advantages_per)."""
+    if advantages.device != logprobs.device:
+        raise ValueError(f"expected advantages on {logprobs.device}, got {advantages.device}")
+    if not advantages.is_floating_point():
+        raise TypeError(f"unsupported advantages dtype: {advantages.dtype}")
+    token = advantages.shape == logprobs.shape
+    if logprobs.ndim == 2:
+        seq = advantages.shape in ((lay.seqs,), (lay.seqs, 1))
+    else:
+        seq = advantages.shape == (lay.seqs,)
+    if per == "token":
+        seq = False
+    elif per == "sequence":
+        token = False
+    if not token and not seq:
+        raise ValueError(
+            f"expected advantages per token {tuple(logprobs.shape)} or per sequence {(lay.seqs,)}, "
+            f"got {tuple(advantages.shape)}"
+        )
+    code = 1 if not token else 2 if seq and lay.cu is not None else 0
+    return advantages.to(torch.float32).contiguous(), code
+
+
+def policy_loss_forward(
+    logprobs: Tensor,
+    old_logprobs: Tensor | None,
+    advantages: Tensor,
+    ref_logprobs: Tensor | None,
+    mask: Tensor | None,
+    cu_seqlens: Tensor | None,
+    clip_low: float,
+    clip_high: float,
+    kl_multiplier: float,
+    reduction: str,
+    advantages_per: str = "auto",
+    want_grad: bool = True,
+) -> tuple[Tensor, Tensor, Tensor | None, Tensor]:
+    """``(loss, stats, dlogprobs or None, workspace)``.
+
+    ``stats`` (fp32): mean KL estimate, share of clipped tokens, valid tokens,
+    weight of a token. ``dlogprobs`` (fp32, unweighted), ``stats`` and the
+    workspace are what ``policy_loss_backward`` needs.
+    """
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"Unsupported reduction: {reduction}")
+    if advantages_per not in ADVANTAGES_PER:
+        raise ValueError(f"advantages_per must be 'auto', 'token' or 'sequence', got {advantages_per!r}")
+    if not (clip_low >= 0.0 and clip_high >= 0.0):
+        raise ValueError(f"clip_low and clip_high must not be negative, got {clip_low} and {clip_high}")
+    if not math.isfinite(kl_multiplier):
+        raise ValueError(f"kl_multiplier must be finite, got {kl_multiplier}")
+    if kl_multiplier != 0.0 and ref_logprobs is None:
+        raise ValueError("kl_multiplier needs ref_logprobs")
+    for name, t in (("old_logprobs", old_logprobs), ("ref_logprobs", ref_logprobs)):
+        if t is not None:
+            _check_like(name, t, logprobs)
+    lay = _layout(logprobs, mask, cu_seqlens)
+    adv, per = _advantages(advantages, logprobs, lay, advantages_per)
+    other, (old, ref) = _others(logprobs, old_logprobs, ref_logprobs)
+    dev = logprobs.device
+    red = REDUCTIONS[reduction]
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.raise_pending(dev, "clipped_policy_loss")
+        lp = logprobs.contiguous()
+        m = None if mask is None else mask.contiguous()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        stats = torch.empty(4, dtype=torch.float32, device=dev)
+        d = torch.empty(lay.tokens, dtype=torch.float32, device=dev) if want_grad else None
+        ws = _lib.workspace(lib.gh_policy_loss_workspace_bytes(lay.tokens, lay.seqs, red), dev)
+        st = lib.gh_policy_loss_fwd(
+            lp.data_ptr(), _lib.dtype_code(lp.dtype), _lib.ptr(old), _lib.ptr(ref), other, adv.data_ptr(), per,
+            _lib.ptr(m), lay.tokens, _lib.ptr(lay.cu), lay.cu_code, lay.seqs, float(clip_low), float(clip_high),
+            float(kl_multiplier), red, loss.data_ptr(), stats.data_ptr(), _lib.ptr(d), stats.data_ptr() + 12,
+            ws.data_ptr(), ws.numel(), _lib.stream_of(lp),
+        )
+        _lib.check(st, "clipped_policy_loss")
+        _lib.raise_on_report(dev, "clipped_policy_loss")
+    return loss, stats, d, ws
+
+
+def policy_loss_backward(
+    dlogprobs: Tensor,
+    stats: Tensor,
+    workspace: Tensor,
+    cu_seqlens: Tensor | None,
+    grad_output: Tensor,
+    shape: list[int] | torch.Size,
+    dtype: torch.dtype,
+    reduction: str,
+) -> Tensor:
+    """``grad_output * dloss/dlogprobs`` in ``shape`` and ``dtype``."""
+    dev = dlogprobs.device
+    tokens = dlogprobs.numel()
+    seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None else shape[0] if len(shape) == 2 else 1
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.raise_pending(dev, "clipped_policy_loss backward")
+        grad = torch.empty(shape, dtype=dtype, device=dev)
+        g = grad_output.to(torch.float32)
+        st = lib.gh_policy_loss_bwd(
+            dlogprobs.data_ptr(), stats.data_ptr() + 12, workspace.data_ptr(), workspace.numel(), g.data_ptr(),
+            tokens, _lib.ptr(cu_seqlens), 0 if cu_seqlens is None else _lib.dtype_code(cu_seqlens.dtype), seqs,
+            REDUCTIONS[reduction], grad.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(dlogprobs),
+        )
+        _lib.check(st, "clipped_policy_loss backward")
+    return grad
+
+
+def preference_loss_forward(
+    logprobs: Tensor,
+    ref_logprobs: Tensor | None,
+    mask: Tensor | None,
+    cu_seqlens: Tensor | None,
+    beta: float,
+    loss_type: str,
+    label_smoothing: float,
+    margin: float,
+    length_normalized: bool,
+    reduction: str,
+) -> tuple[Tensor, Tensor, Tensor]:
+    """``(loss, rewards [sequences], gradient of a valid token [sequences])``, all fp32."""
+    if reduction not in ("mean", "sum"):
+        raise ValueError(f"Unsupported reduction: {reduction}")
+    if loss_type not in KINDS:
+        raise ValueError(f"loss_type must be 'sigmoid', 'hinge' or 'ipo', got {loss_type!r}")
+    if not (beta > 0.0 and math.isfinite(beta)):
+        raise ValueError(f"beta must be positive and finite, got {beta}")
+    if not math.isfinite(margin):
+        raise ValueError(f"margin must be finite, got {margin}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must lie in [0, 1], got {label_smoothing}")
+    if label_smoothing != 0.0 and loss_type != "sigmoid":
+        raise ValueError("label_smoothing goes with loss_type='sigmoid'")
+    if ref_logprobs is not None:
+        _check_like("ref_logprobs", ref_logprobs, logprobs)
+    if logprobs.ndim == 1 and cu_seqlens is None:
+        raise ValueError("packed logprobs need cu_seqlens")
+    seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None and cu_seqlens.ndim == 1 else logprobs.shape[0]
+    if seqs % 2:
+        raise ValueError(f"expected an even number of sequences (the chosen, then the rejected ones), got {seqs}")
+    lay = _layout(logprobs, mask, cu_seqlens)
+    other, (ref,) = _others(logprobs, ref_logprobs)
+    dev = logprobs.device
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.raise_pending(dev, "preference_loss")
+        lp = logprobs.contiguous()
+        m = None if mask is None else mask.contiguous()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        rewards = torch.empty(lay.seqs, dtype=torch.float32, device=dev)
+        coef = torch.empty(lay.seqs, dtype=torch.float32, device=dev)
+        ws = _lib.workspace(lib.gh_preference_loss_workspace_bytes(lay.tokens, lay.seqs), dev)
+        st = lib.gh_preference_loss_fwd(
+            lp.data_ptr(), _lib.dtype_code(lp.dtype), _lib.ptr(ref), other, _lib.ptr(m), lay.tokens,
+            _lib.ptr(lay.cu), lay.cu_code, lay.seqs, float(beta), float(margin), float(label_smoothing),
+            KINDS[loss_type], int(length_normalized), int(reduction == "mean"), loss.data_ptr(), rewards.data_ptr(),
+            coef.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(lp),
+        )
+        _lib.check(st, "preference_loss")
+        _lib.raise_on_report(dev, "preference_loss")
+    return loss, rewards, coef
+
+
+def preference_loss_backward(
+    coef: Tensor,
+    grad_output: Tensor,
+    mask: Tensor | None,
+    cu_seqlens: Tensor | None,
+    shape: list[int] | torch.Size,
+    dtype: torch.dtype,
+) -> Tensor:
+    """``grad_output * dloss/dlogprobs`` in ``shape`` and ``dtype``."""
+    dev = coef.device
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.raise_pending(dev, "preference_loss backward")
+        grad = torch.empty(shape, dtype=dtype, device=dev)
+        g = grad_output.to(torch.float32)
+        m = None if mask is None else mask.contiguous()
+        cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+        st = lib.gh_preference_loss_bwd(
+            coef.data_ptr(), g.data_ptr(), _lib.ptr(m), grad.numel(), _lib.ptr(cu),
+            0 if cu is None else _lib.dtype_code(cu.dtype), coef.numel(), grad.data_ptr(), _lib.dtype_code(dtype),
+            _lib.stream_of(grad),
+        )
+        _lib.check(st, "preference_loss backward")
+    return grad

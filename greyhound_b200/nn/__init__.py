@@ -1,3 +1,3 @@
-from greyhound_b200.nn import functional
+from greyhound_b200.nn import functional, utils
 
-__all__ = ["functional"]
+__all__ = ["functional", "utils"]

@@ -3,7 +3,8 @@
 ``selective_log_softmax`` (:53-69), ``cross_entropy`` (:72-116),
 ``autograd_loss_and_logits_grad`` (:119-148), ``chunked_linear_loss`` (:151-223)
 and ``chunked_linear_cross_entropy`` (:226-287).
-``chunked_linear_selective_log_softmax`` has no counterpart there. ``weight`` is ``[V, D]`` and is
+``chunked_linear_selective_log_softmax``, ``clipped_policy_loss`` and
+``preference_loss`` have no counterpart there. ``weight`` is ``[V, D]`` and is
 handed to the ops as the ``[D, V]`` view ``weight.T``, exactly as the reference
 does, so the op schemas and their fakes are unchanged.
 """
@@ -11,7 +12,7 @@ does, so the op schemas and their fakes are unchanged.
 from __future__ import annotations
 
 from collections.abc import Callable
-from typing import Any, Literal, cast
+from typing import Any, Literal, NamedTuple, cast
 
 import torch
 from torch import Tensor
@@ -20,7 +21,9 @@ from greyhound_b200.ops.chunked_linear_cross_entropy import ChunkedLinearCrossEn
 from greyhound_b200.ops.chunked_linear_loss import ChunkedLinearLossFunction
 from greyhound_b200.ops.chunked_linear_selective_log_softmax import ChunkedLinearSelectiveLogSoftmaxFunction
 from greyhound_b200.ops.cross_entropy import CrossEntropyFunction
+from greyhound_b200.kernels.token_losses import _no_grad_to
 from greyhound_b200.ops.logprobs import SelectiveLogSoftmaxFunction
+from greyhound_b200.ops.token_losses import ClippedPolicyLossFunction, PreferenceLossFunction
 
 __all__ = [
     "selective_log_softmax",
@@ -29,7 +32,26 @@ __all__ = [
     "chunked_linear_loss",
     "chunked_linear_cross_entropy",
     "chunked_linear_selective_log_softmax",
+    "clipped_policy_loss",
+    "preference_loss",
+    "PolicyLossMetrics",
+    "PreferenceRewards",
 ]
+
+
+class PolicyLossMetrics(NamedTuple):
+    """0-d fp32 tensors over the valid tokens, without gradients."""
+
+    kl: Tensor  # mean of e^u - u - 1, u = ref - logprob (0 without ref_logprobs)
+    clip_fraction: Tensor  # share of tokens whose ratio is clipped
+    tokens: Tensor  # their number
+
+
+class PreferenceRewards(NamedTuple):
+    """``[pairs]`` fp32 tensors, without gradients: beta times each sequence's log ratio."""
+
+    chosen: Tensor
+    rejected: Tensor
 
 
 def _slice_chunk_arg(value: Any, start: int, end: int, batch_size: int) -> Any:
@@ -206,3 +228,96 @@ def chunked_linear_selective_log_softmax(
         ),
     )
     return flat.reshape(index.shape)
+
+
+def clipped_policy_loss(
+    logprobs: Tensor,
+    old_logprobs: Tensor | None,
+    advantages: Tensor,
+    ref_logprobs: Tensor | None = None,
+    mask: Tensor | None = None,
+    cu_seqlens: Tensor | None = None,
+    clip_low: float = 0.2,
+    clip_high: float = 0.2,
+    kl_multiplier: float = 0.0,
+    reduction: Literal["sum", "mean", "sequence_mean"] = "mean",
+    advantages_per: Literal["auto", "token", "sequence"] = "auto",
+    return_metrics: bool = False,
+) -> Tensor | tuple[Tensor, PolicyLossMetrics]:
+    """Clipped policy loss, with a KL term towards a reference policy.
+
+    Per token, with ``r = exp(logprobs - old_logprobs)``, ``A`` the advantage and
+    ``u = ref_logprobs - logprobs``::
+
+        -min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A) + kl_multiplier * (exp(u) - u - 1)
+
+    ``logprobs`` (as from ``selective_log_softmax`` or
+    ``chunked_linear_selective_log_softmax``; fp16, bf16 or fp32) are padded
+    ``[sequences, length]`` or packed ``[tokens]`` with ``cu_seqlens``
+    ``[sequences + 1]`` (int32 / int64; without it, all tokens are one sequence).
+    ``mask`` (bool, like ``logprobs``) is True on the tokens that count; what the
+    others hold is never used. ``old_logprobs=None`` stands for ``logprobs``
+    themselves (ratio 1, with its gradient). ``advantages`` come per token or
+    per sequence (``[sequences]``, padded also ``[sequences, 1]``); where packed
+    tokens are as many as sequences, ``"auto"`` takes one token per sequence, and
+    anything else has to say ``advantages_per``.
+
+    ``reduction``: ``"sum"``, ``"mean"`` over the valid tokens, or
+    ``"sequence_mean"``, the mean over the sequences that have valid tokens of
+    the mean over each's. No valid token gives 0.
+
+    Returns the fp32 loss, differentiable once with respect to ``logprobs``
+    alone; with ``return_metrics`` also ``PolicyLossMetrics``.
+    """
+    _no_grad_to(old_logprobs=old_logprobs, advantages=advantages, ref_logprobs=ref_logprobs)
+    loss, stats = ClippedPolicyLossFunction.apply(
+        logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, float(clip_low), float(clip_high),
+        float(kl_multiplier), reduction, advantages_per,
+    )
+    if not return_metrics:
+        return cast(Tensor, loss)
+    return loss, PolicyLossMetrics(stats[0], stats[1], stats[2])
+
+
+def preference_loss(
+    logprobs: Tensor,
+    ref_logprobs: Tensor | None = None,
+    mask: Tensor | None = None,
+    cu_seqlens: Tensor | None = None,
+    beta: float = 0.1,
+    loss_type: Literal["sigmoid", "hinge", "ipo"] = "sigmoid",
+    label_smoothing: float = 0.0,
+    margin: float = 0.0,
+    length_normalized: bool = False,
+    reduction: Literal["sum", "mean"] = "mean",
+    return_rewards: bool = False,
+) -> Tensor | tuple[Tensor, PreferenceRewards]:
+    """Preference loss of paired sequences from their tokens' log-probabilities.
+
+    The first half of the sequences are the chosen ones, the second half the
+    rejected ones, in the same order. With ``s`` a sequence's sum over its valid
+    tokens of ``logprobs - ref_logprobs`` (``None``: 0), divided by their number
+    if ``length_normalized``, ``h = s_chosen - s_rejected`` and
+    ``z = beta * h - margin``::
+
+        sigmoid   -(1 - e) * log sigmoid(z) - e * log sigmoid(-z),  e = label_smoothing
+        hinge     max(0, 1 - z)
+        ipo       (h - margin - 1 / (2 * beta)) ** 2
+
+    summed over the pairs or averaged. ``logprobs`` are padded
+    ``[sequences, length]`` or packed ``[tokens]`` with ``cu_seqlens``
+    ``[sequences + 1]``; ``mask`` (bool) is True on the tokens that count. A
+    sequence without any has ``s = 0``.
+
+    Returns the fp32 loss, differentiable once with respect to ``logprobs``
+    alone; with ``return_rewards`` also ``PreferenceRewards``.
+    """
+    _no_grad_to(ref_logprobs=ref_logprobs)
+    loss, rewards = PreferenceLossFunction.apply(
+        logprobs, ref_logprobs, mask, cu_seqlens, float(beta), loss_type, float(label_smoothing), float(margin),
+        bool(length_normalized), reduction,
+    )
+    if not return_rewards:
+        return cast(Tensor, loss)
+    pairs = rewards.shape[0] // 2
+    return loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])

@@ -1,0 +1,98 @@
+"""Gradient norm and clipping over many tensors.
+
+``clip_grad_norm_`` takes what ``torch.nn.utils.clip_grad_norm_`` takes, without a
+host sync and in two launches; ``clip_by_global_norm`` is the form for a list of
+tensors that need not belong to parameters, in place or not.
+"""
+
+from __future__ import annotations
+
+import math
+from collections.abc import Iterable, Sequence
+
+import torch
+from torch import Tensor
+
+from greyhound_b200.kernels.grad_norm import clip_tensors
+
+__all__ = ["clip_by_global_norm", "clip_grad_norm_", "global_norm"]
+
+
+def _device(tensors: Sequence[Tensor]) -> torch.device:
+    if tensors:
+        return tensors[0].device
+    return torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else torch.device("cpu")
+
+
+def global_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
+    """Norm of all elements of ``tensors`` together, a 0-d fp32 tensor.
+
+    ``norm_type`` is 2.0 or ``inf`` (the largest absolute value). Tensors are
+    fp16, bf16 or fp32, on one device, mixed as they come; a tensor listed
+    twice counts twice. Squares are summed in fp64.
+    """
+    ts = [t.detach() for t in tensors]
+    if not ts:
+        return torch.zeros((), dtype=torch.float32, device=_device(ts))
+    return clip_tensors(ts, None, 0.0, float(norm_type), _device(ts))
+
+
+def clip_by_global_norm(
+    tensors: Iterable[Tensor],
+    max_norm: float,
+    norm_type: float = 2.0,
+    out: Iterable[Tensor] | None = None,
+) -> tuple[list[Tensor], Tensor]:
+    """``(clipped, norm)``: every tensor times ``min(1, max_norm / (norm + 1e-6))``.
+
+    ``norm`` is ``global_norm(tensors)`` before clipping. ``out`` gives the
+    tensors to write, of the same shapes and types: new ones by default, or
+    ``tensors`` themselves for clipping in place, which writes nothing when the
+    norm is below ``max_norm``. Outputs may not overlap each other or another
+    tensor's input (``ValueError``). A NaN norm makes every element NaN, an
+    infinite one makes finite elements 0, as the formula says.
+    """
+    ts = [t.detach() for t in tensors]
+    given = None if out is None else [t.detach() for t in out]
+    # the same tensor given for both is clipped in place
+    if given is not None and len(given) == len(ts):
+        given = [
+            t if o.data_ptr() == t.data_ptr() and o.shape == t.shape and o.stride() == t.stride()
+            and o.dtype == t.dtype else o
+            for o, t in zip(given, ts)
+        ]
+    outs = [torch.empty_like(t) for t in ts] if given is None else given
+    if not ts:
+        if outs:
+            raise ValueError(f"expected 0 outputs, got {len(outs)}")
+        return [], torch.zeros((), dtype=torch.float32, device=_device(ts))
+    return outs, clip_tensors(ts, outs, float(max_norm), float(norm_type), _device(ts))
+
+
+def clip_grad_norm_(
+    parameters: Tensor | Iterable[Tensor],
+    max_norm: float,
+    norm_type: float = 2.0,
+    error_if_nonfinite: bool = False,
+) -> Tensor:
+    """Clip the gradients of ``parameters`` in place to a global norm of ``max_norm``.
+
+    Returns the norm before clipping (0-d fp32, on the device). Parameters
+    without a gradient do not count. The gradients are scaled by
+    ``min(1, max_norm / (norm + 1e-6))`` computed on the device: the call does
+    not synchronise, except with ``error_if_nonfinite``, which reads the norm
+    and raises ``RuntimeError`` before any gradient has changed.
+    Two parameters that share their gradient's memory raise ``ValueError``.
+    """
+    if isinstance(parameters, Tensor):
+        parameters = [parameters]
+    grads = [p.grad.detach() for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device=_device(grads))
+    if not float(max_norm) >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if error_if_nonfinite:
+        norm = clip_tensors(grads, None, 0.0, float(norm_type), _device(grads))
+        if not math.isfinite(norm.item()):
+            raise RuntimeError(f"the norm of the gradients is {norm.item()}; they were not clipped")
+    return clip_tensors(grads, grads, float(max_norm), float(norm_type), _device(grads))

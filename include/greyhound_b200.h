@@ -54,9 +54,12 @@ enum {
   GH_EUNSUPPORTED = 5
 };
 
-/* device-side status bits written into the workspace status word */
+/* device-side status bits written into the workspace status word (or, where a
+ * call has none, straight into the device's sticky slot) */
 enum {
-  GH_DEV_BAD_LABEL = 1   /* a non-ignored label/index outside [0, V) */
+  GH_DEV_BAD_LABEL = 1,  /* a non-ignored label/index outside [0, V) */
+  GH_DEV_BAD_SEQLENS = 2, /* sequence offsets that decrease or leave [0, tokens] */
+  GH_DEV_AMBIGUOUS = 8   /* per-token or per-sequence values? (gh_policy_loss_fwd) */
 };
 
 GH_API int gh_abi_version(void);
@@ -361,6 +364,76 @@ GH_API int gh_lsm_bwd(const void* H, const void* W, const void* index, int index
                       int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
                       int fp32_grad_weight_accum, void* grad_input, void* grad_weight, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * Losses over per-token log-probabilities (no counterpart in the reference).
+ * Tokens lie in `seqs` sequences: padded, of tokens / seqs each, when
+ * cu_seqlens is NULL, otherwise packed, sequence s being [cu[s], cu[s + 1]) of
+ * cu_seqlens [seqs + 1] in {I32, I64}. Offsets that decrease or leave
+ * [0, tokens] set GH_DEV_BAD_SEQLENS in the device's sticky slot; the results
+ * are then unspecified. mask [tokens] (bytes, optional): 0 leaves a token out,
+ * whatever its values; a token outside every sequence is left out, too, and
+ * the gradient of one left out is 0.
+ * logprobs [tokens] in {F16, BF16, F32}; the other log-probabilities in the same
+ * type or F32 (other_dtype). Results are F32 scalars unless stated.
+ *
+ * Clipped policy loss: with d = logprob - old (old NULL: 0), r = e^d,
+ * u = ref - logprob, A the advantage (advantages_per 0: [tokens]; 1: [seqs]; 2:
+ * [tokens] that are as many as the sequences, each of which has to hold one
+ * token, otherwise GH_DEV_AMBIGUOUS is set)
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_multiplier (e^u - u - 1)
+ * (the KL term only with ref_logprobs). reduction: 0 sum, 1 mean over the
+ * valid tokens, 2 mean over the sequences that have any of their valid
+ * tokens' means. metrics[3]: mean of e^u - u - 1, share of clipped tokens,
+ * valid tokens. dlogprobs [tokens] (optional) <- dl/dlogprob, scal[1] and the
+ * workspace: what gh_policy_loss_bwd reads to write
+ * grad [tokens] = grad_output * dloss/dlogprob in logprobs' type.
+ * ------------------------------------------------------------------------ */
+GH_API size_t gh_policy_loss_workspace_bytes(int64_t tokens, int64_t seqs, int reduction);
+GH_API int gh_policy_loss_fwd(const void* logprobs, int dtype, const void* old_logprobs, const void* ref_logprobs,
+                              int other_dtype, const float* advantages, int advantages_per,
+                              const uint8_t* mask, int64_t tokens, const void* cu_seqlens, int cu_dtype,
+                              int64_t seqs, double clip_low, double clip_high, double kl_multiplier, int reduction,
+                              float* loss, float* metrics, float* dlogprobs, float* scal, void* workspace,
+                              size_t workspace_bytes, void* stream);
+GH_API int gh_policy_loss_bwd(const float* dlogprobs, const float* scal, const void* workspace,
+                              size_t workspace_bytes, const float* grad_output, int64_t tokens,
+                              const void* cu_seqlens, int cu_dtype, int64_t seqs, int reduction, void* grad,
+                              int dtype, void* stream);
+
+/* Preference loss over pairs: sequences 0 .. P-1 are chosen, P .. 2P-1 rejected
+ * (seqs = 2P). With s_j the sum over a sequence's valid tokens of
+ * logprob - ref (ref NULL: 0), divided by their number if length_normalized,
+ * h = s_chosen - s_rejected and z = beta h - margin, kind is
+ *   0 (1 - e) softplus(-z) + e softplus(z), e = label_smoothing
+ *   1 max(0, 1 - z)
+ *   2 (h - margin - 1 / (2 beta))^2
+ * summed over the pairs or averaged. rewards [seqs] <- beta s_j; coef [seqs] <-
+ * the gradient of a valid token of each sequence, which gh_preference_loss_bwd
+ * spreads over the tokens, times grad_output, in logprobs' type. */
+GH_API size_t gh_preference_loss_workspace_bytes(int64_t tokens, int64_t seqs);
+GH_API int gh_preference_loss_fwd(const void* logprobs, int dtype, const void* ref_logprobs, int other_dtype,
+                                  const uint8_t* mask, int64_t tokens, const void* cu_seqlens, int cu_dtype,
+                                  int64_t seqs, double beta, double margin, double label_smoothing, int kind,
+                                  int length_normalized, int mean_reduction, float* loss, float* rewards,
+                                  float* coef, void* workspace, size_t workspace_bytes, void* stream);
+GH_API int gh_preference_loss_bwd(const float* coef, const float* grad_output, const uint8_t* mask, int64_t tokens,
+                                  const void* cu_seqlens, int cu_dtype, int64_t seqs, void* grad, int dtype,
+                                  void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * Norm of all elements of `count` dense tensors in {F16, BF16, F32} (host
+ * arrays of device pointers, element counts and dtype codes): 2-norm, or with
+ * inf_norm the largest absolute value, to *norm (device F32); and, unless
+ * outputs is NULL, outputs[i] = min(1, max_norm / (norm + 1e-6)) * tensors[i] in
+ * the tensor's type. outputs[i] may be tensors[i]; otherwise outputs overlap
+ * neither inputs nor each other (GH_EINVAL). The arrays are read before the
+ * call returns.
+ * ------------------------------------------------------------------------ */
+GH_API size_t gh_global_norm_workspace_bytes(int64_t count);
+GH_API int gh_clip_by_global_norm(const void* const* tensors, void* const* outputs, const int64_t* numels,
+                                  const int* dtypes, int64_t count, double max_norm, int inf_norm, float* norm,
+                                  void* workspace, size_t workspace_bytes, void* stream);
 
 /* Optional event timing of the library's launches, by kernel class:
  * 0 logits GEMM + fused CE epilogue, 1 dW GEMM, 2 dH GEMM, 3 dlogits pass,
