@@ -5,7 +5,7 @@
 //
 // Two launches for up to kMaxTensors tensors whatever their number and sizes:
 // the list travels as a kernel argument (no copy to the device, so the calls
-// can be captured), tensors are cut into chunks of kChunk elements, and blocks
+// can be captured), tensors are cut into chunks of kChunkBytes, and blocks
 // take chunks round-robin. The first kernel leaves one partial per block; every
 // block of the second sums those partials itself, in the same order, instead
 // of waiting for a last block, then scales its chunks from the last one
@@ -28,7 +28,9 @@ namespace gh {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int64_t kChunk = 16384;  // elements
+// Four 32-byte vectors for each of a block's threads, all in flight at once
+// (at two, half as much, the bf16 norm of 2.3 GB ran at 5.1 TB/s).
+constexpr int64_t kChunkBytes = (int64_t)kThreads * 4 * 32;
 
 template <int MAX>
 struct List {
@@ -59,13 +61,14 @@ __device__ __forceinline__ int tensor_of(const List<MAX>& l, int chunk) {
 // multiple of 32 bytes, so only a tensor's ends have scalars beside vectors.
 __device__ __forceinline__ void chunk_range(const void* base, int elt, int64_t n, int64_t c, int64_t* a, int64_t* b) {
   const int64_t mis = (int64_t)(reinterpret_cast<uintptr_t>(base) & 31) / elt;
-  int64_t s = c * kChunk - mis, e = s + kChunk;
+  const int64_t chunk = kChunkBytes / elt;
+  int64_t s = c * chunk - mis, e = s + chunk;
   *a = s < 0 ? 0 : s;
   *b = e < n ? e : n;
 }
 inline int64_t chunks_of(const void* base, int elt, int64_t n) {
   const int64_t mis = (int64_t)(reinterpret_cast<uintptr_t>(base) & 31) / elt;
-  return n == 0 ? 0 : (mis + n + kChunk - 1) / kChunk;
+  return n == 0 ? 0 : ((mis + n) * elt + kChunkBytes - 1) / kChunkBytes;
 }
 
 // Accumulators: sum of squares in fp64, or the largest |x| as bits (a NaN's

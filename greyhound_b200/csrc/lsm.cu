@@ -232,8 +232,100 @@ lsm_clean_rows_kernel(const uint4* __restrict__ H, const int* __restrict__ tgt, 
     st16(out + i, tgt[i / vpr] >= 0 ? ld16(H + i) : make_uint4(0, 0, 0, 0));
 }
 
+// out = row[r] * scale * sum_s part[s][r][c], the slices of a split-K product.
+template <typename T>
+__global__ void __launch_bounds__(256)
+lsm_join_kernel(const float* __restrict__ part, int slices, int64_t n, int64_t D, const float* __restrict__ row,
+                const float* __restrict__ scale, T* __restrict__ out) {
+  const float f = scale ? *scale : 1.f;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+    float4 a = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll 4
+    for (int s = 1; s < slices; ++s) {
+      const float4 b = *reinterpret_cast<const float4*>(part + s * n + i);
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    const float g = row ? f * row[i / D] : f;
+    T o[4] = {Elt<T>::from_f(a.x * g), Elt<T>::from_f(a.y * g), Elt<T>::from_f(a.z * g), Elt<T>::from_f(a.w * g)};
+    *reinterpret_cast<uint2*>(out + i) = *reinterpret_cast<const uint2*>(o);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host side
+
+// K slices of the dH product [rows, D] over K = V. Its few output tiles leave
+// most SMs idle at a few hundred rows (512 x 1024 over 32000: 8 pair tiles for 74
+// pairs of SMs, 157 us), while K is long: the slices' fp32 sums are written to
+// memory and joined. Modelled in us: 0.38 a k-step of a 256 x 256 pair tile
+// (measured at full load), 12 k-steps a tile for its ends, the slices' traffic
+// at 5 TB/s. 0: run_gemm's own choice (two 16-bit halves at most) is as good.
+int dh_slices(int64_t rows, int64_t D, int64_t V) {
+  const int pair = pick_pair(rows);
+  const int64_t units = num_sms_dev() / pair;
+  const int64_t tiles = (rows + BM * pair - 1) / (BM * pair) * ((D + BN - 1) / BN);
+  const int64_t nkb = (V + BK - 1) / BK;
+  auto waves = [&](int64_t t) { return (double)((t + units - 1) / units); };
+  double best = 0.9 * (nkb >= 32 && pair == 2 && D > BN ? waves(tiles) * ((double)nkb / 2 + 12) * 0.72 + 4.0
+                                                       : waves(tiles) * ((double)nkb + 12) * 0.38);
+  int slices = 0;
+  for (int s = 2; s <= 64 && nkb / s >= 8; ++s) {
+    const int64_t per = (nkb + s - 1) / s, n = (nkb + per - 1) / per;  // no empty slice
+    if (n != s) continue;
+    const double t = waves(tiles * s) * ((double)per + 12) * 0.38 + (double)s * rows * D * 8 / 5e6 + 4.0;
+    if (t < best) {
+      best = t;
+      slices = s;
+    }
+  }
+  return slices;
+}
+
+// Bytes of the second product's scratch: the slices in fp32, or run_gemm's
+// second 16-bit half.
+size_t dh_scratch(int64_t rows, int64_t D, int64_t V) {
+  const int s = dh_slices(rows, D, V);
+  return (size_t)rows * D * (s ? (size_t)s * 4 : 2);
+}
+
+// dH[rows, D] = row[r] * scale * (A[rows, V] W[V, D]).
+template <typename T>
+int dh_gemm(int dtype, const Operand& A, const void* W, int64_t rows, int64_t D, int64_t V, void* out,
+            const float* scale, const float* row, void* scratch, int* status, cudaStream_t st) {
+  const int slices = dh_slices(rows, D, V);
+  const int sms = num_sms_dev();
+  const Operand B{W, D, 1};
+  if (!slices)  // fp16: two 16-bit halves would round twice, near zero by a step each
+    return run_gemm(dtype, A, B, rows, D, V, out, dtype, D, nullptr, nullptr, 0, scale, 1, sms, st, status,
+                    PROF_GEMM_DH, Hints{}, dtype == GH_F16 ? nullptr : scratch, row);
+  const int pair = pick_pair(rows);
+  CUtensorMap ta, tb;
+  int rc = make_operand_maps(&ta, &tb, dtype, A, B, rows, D, V, pair);
+  if (rc) return rc;
+  gemm::Params p{};
+  set_tiles(p, rows, D, V, pair, 1, slices);
+  p.raster = 1;
+  p.group = 1;
+  p.out = scratch;
+  p.ldo = D;
+  p.vec_ok = 1;
+  p.split_bytes = (int64_t)rows * D * 4;
+  p.status = status;
+  {
+    ProfScope prof(PROF_GEMM_DH, st);
+    rc = pair == 2 ? launch_gemm_t<T, 0, 1, gemm::EPI_STORE, float, 2>(ta, tb, p, sms, st)
+                   : launch_gemm_t<T, 0, 1, gemm::EPI_STORE, float, 1>(ta, tb, p, sms, st);
+    if (rc) return rc;
+  }
+  const int64_t n = rows * D, want = (n + 1023) / 1024, cap = 8 * (int64_t)sms;
+  lsm_join_kernel<T><<<(unsigned)(want < cap ? want : cap), 256, 0, st>>>(static_cast<const float*>(scratch), slices, n,
+                                                                        D, row, scale, static_cast<T*>(out));
+  count_launch(1);
+  return check_launch("lsm_join");
+}
 
 struct FwdLayout {
   size_t status = 0, tgt, xt, lse2, rowflag, stats, qmode, gmax, total;
@@ -290,7 +382,10 @@ BwdLayout bwd_layout(int64_t N, int64_t D, int64_t V, int64_t chunk, bool kept, 
   L.tval = off; off = al256(off + (kept ? 0 : sizeof(float) * N));
   L.d = off;    off = al256(off + (kept ? 0 : (size_t)chunk * L.ldd * 2));
   L.hs = off;   off = al256(off + (size_t)chunk * D * 2);
-  L.dh2 = off;  off = al256(off + (size_t)chunk * D * 2);
+  // the last chunk may be shorter and take more slices of fewer rows
+  const int64_t rest = N > 0 ? N - (N - 1) / chunk * chunk : 0;
+  const size_t a = dh_scratch(chunk, D, V), b = dh_scratch(rest, D, V);
+  L.dh2 = off;  off = al256(off + (a > b ? a : b));
   L.need_acc = !kept && fp32_accum && N > chunk;
   L.acc = off;
   if (L.need_acc) off = al256(off + sizeof(float) * (size_t)D * V);
@@ -412,8 +507,8 @@ int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N,
   if (dW && (rc = run_gemm(GH_BF16, Operand{kept + K.q, K.ldq, 1}, Operand{hs, D, 1}, V, D, N, dW, GH_BF16, D, nullptr,
                            nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
     return rc;
-  if (dH && (rc = run_gemm(GH_BF16, Operand{kept + K.q, K.ldq, 0}, Operand{W, D, 1}, N, D, V, dH, GH_BF16, D, nullptr,
-                           nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DH, Hints{}, ws + L.dh2, a)))
+  if (dH && (rc = dh_gemm<__nv_bfloat16>(GH_BF16, Operand{kept + K.q, K.ldq, 0}, W, N, D, V, dH, nullptr, a,
+                                         ws + L.dh2, status, st)))
     return rc;
   return publish_status(status, st);
 }
@@ -477,9 +572,8 @@ int lsm_bwd_run(const void* H, const void* W, const float* y, const float* lse2,
                          add_same, D, unscale, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
         return rc;
     }
-    if (dH && (rc = run_gemm(dtype, Operand{d, L.ldd, 0}, Operand{W, D, 1}, rows, D, V, static_cast<T*>(dH) + s0 * D,
-                             dtype, D, nullptr, nullptr, 0, unscale, 1, sms, st, status, PROF_GEMM_DH, Hints{},
-                             ws + L.dh2)))
+    if (dH && (rc = dh_gemm<T>(dtype, Operand{d, L.ldd, 0}, W, rows, D, V, static_cast<T*>(dH) + s0 * D, unscale,
+                               nullptr, ws + L.dh2, status, st)))
       return rc;
   }
   return publish_status(status, st);

@@ -80,6 +80,9 @@ struct Params {
   // slice 0 writes `out`, slice 1 writes `out2` (same pitch), the host sums
   int ksplit;
   void* out2;
+  // > 0 (256-column tiles): slice s writes at out + s * split_bytes instead, for
+  // any number of slices; every slice holds at least one 64-wide k-step
+  int64_t split_bytes;
   int vec_ok;           // 16-byte aligned rows (vector stores allowed)
   const float* add_f32; // optional fp32 addend [M, ldadd]
   const void* add_same; // optional addend in the output type [M, ldadd]
@@ -690,7 +693,9 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     for (int tile = unit; tile < p.num_tiles && !stop; tile += nunits) {
       const TileK tk = tile_k(p, tile, nkb);
       const int mt = tk.mt, nt = tk.nt;
-      void* const pout = tk.ks ? p.out2 : p.out;  // this K slice's output
+      // this K slice's output
+      void* const pout = NSUB == 1 && p.split_bytes ? static_cast<char*>(p.out) + tk.ks * p.split_bytes
+                         : tk.ks ? p.out2 : p.out;
       const int m0 = mt * G::TM + (int)rank * BM;
       if (NSUB == 1) {
         if (!tc::mbar_wait(&tfull[acc], acc_phase, abort_flag, lim)) break;

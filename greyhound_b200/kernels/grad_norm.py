@@ -3,8 +3,9 @@ the C-ABI): two launches for up to 896 tensors, whatever their sizes."""
 
 from __future__ import annotations
 
-import ctypes
 import math
+import operator
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -27,17 +28,65 @@ def is_dense(t: Tensor) -> bool:
     return True
 
 
-def _validate(tensors: Sequence[Tensor], norm_type: float) -> None:
-    if norm_type not in (2.0, math.inf):
-        raise ValueError(f"norm_type must be 2.0 or inf, got {norm_type}")
-    dev = tensors[0].device if tensors else None
-    for i, t in enumerate(tensors):
-        if t.layout != torch.strided:
-            raise TypeError(f"expected dense tensors, got layout {t.layout} at {i}")
-        if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
-            raise TypeError(f"unsupported dtype of tensor {i}: {t.dtype}")
-        if not t.is_cuda or t.device != dev:
-            raise ValueError(f"expected all tensors on one CUDA device, got {t.device} at {i} and {dev} before it")
+_CODES = {torch.float16: _lib.GH_F16, torch.bfloat16: _lib.GH_BF16, torch.float32: _lib.GH_F32}
+
+
+_STRIDED = {torch.strided}
+
+
+def _dense(t: Tensor) -> Tensor:
+    return t if is_dense(t) else t.detach().contiguous()
+
+
+def _refuse(i: int, t: Tensor, dev: torch.device) -> None:
+    if t.layout != torch.strided:
+        raise TypeError(f"expected dense tensors, got layout {t.layout} at {i}")
+    if t.dtype not in _CODES:
+        raise TypeError(f"unsupported dtype of tensor {i}: {t.dtype}")
+    raise ValueError(f"expected all tensors on one CUDA device, got {t.device} at {i} and {dev} before it")
+
+
+def _operands(
+    tensors: Sequence[Tensor], outputs: Sequence[Tensor] | None, device: torch.device
+) -> tuple[array, Sequence[Tensor], Sequence[Tensor] | None, list[tuple[Tensor, Tensor]]]:
+    """(dtype codes, dense inputs, dense outputs, copies to make afterwards)."""
+    # Contiguous tensors on one device, the common list of hundreds: walked by
+    # map over the tensors' methods, which costs less than half of a loop.
+    index = device.index if device.type == "cuda" else None
+    found = list(map(_CODES.get, [t.dtype for t in tensors]))
+    if index is None or None in found or {t.layout for t in tensors} != _STRIDED or set(
+        map(Tensor.get_device, tensors)
+    ) != {index}:
+        for i, t in enumerate(tensors):
+            if t.dtype not in _CODES or t.device != device or t.layout != torch.strided or not t.is_cuda:
+                _refuse(i, t, device)
+    codes = array("i", found)
+    whole = all(map(Tensor.is_contiguous, tensors))
+    if outputs is None:
+        return codes, tensors if whole else [_dense(t) for t in tensors], None, []
+    if all(map(operator.is_, tensors, outputs)):
+        outputs = tensors
+    else:
+        same = all(map(Tensor.is_same_size, tensors, outputs)) and [o.dtype for o in outputs] == [
+            t.dtype for t in tensors
+        ]
+        if not same or {o.layout for o in outputs} != _STRIDED or set(map(Tensor.get_device, outputs)) != {index}:
+            for i, (o, t) in enumerate(zip(outputs, tensors)):
+                if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.layout != torch.strided:
+                    raise ValueError(f"output {i} must match its tensor in shape, dtype and device")
+    if whole and (outputs is tensors or all(map(Tensor.is_contiguous, outputs))):
+        return codes, tensors, outputs, []
+    src, dst = [], []
+    back: list[tuple[Tensor, Tensor]] = []
+    for o, t in zip(outputs, tensors):
+        s = _dense(t)
+        # written in place of the input's dense copy, or where input and output are laid out alike
+        d = s if o is t else o if s is t and o.stride() == t.stride() else torch.empty_like(s)
+        src.append(s)
+        dst.append(d)
+        if d is not o:
+            back.append((o, d))
+    return codes, src, dst, back
 
 
 def clip_tensors(
@@ -50,43 +99,30 @@ def clip_tensors(
     """The norm of all ``tensors`` (0-d fp32); with ``outputs``, also
     ``outputs[i] = min(1, max_norm / (norm + 1e-6)) * tensors[i]``.
 
-    An output has its tensor's shape, type and strides; it may be the tensor."""
-    _validate(tensors, norm_type)
+    An output has its tensor's shape and type; it may be the tensor itself."""
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f"norm_type must be 2.0 or inf, got {norm_type}")
     if outputs is not None:
         if not max_norm >= 0.0:
             raise ValueError(f"max_norm must not be negative, got {max_norm}")
         if len(outputs) != len(tensors):
             raise ValueError(f"expected {len(tensors)} outputs, got {len(outputs)}")
-        for i, (o, t) in enumerate(zip(outputs, tensors)):
-            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
-                raise ValueError(f"output {i} must match its tensor in shape, dtype and device")
+    codes, src, dst, back = _operands(tensors, outputs, device)
     lib = _lib.load()
-    n = len(tensors)
-    with torch.cuda.device(device):
+    n = len(src)
+    with _lib.on_device(device):
         _lib.raise_pending(device, "clip_by_global_norm")
-        # a tensor with gaps, or an output laid out otherwise, goes through dense copies
-        src = [t if is_dense(t) else t.contiguous() for t in tensors]
-        dst = None
-        if outputs is not None:
-            dst = [
-                o if o is t or (o.stride() == s.stride() and (s is t)) else torch.empty_like(s)
-                for o, t, s in zip(outputs, tensors, src)
-            ]
-            dst = [s if (o is t and s is not t) else d for o, t, s, d in zip(outputs, tensors, src, dst)]
         norm = torch.empty((), dtype=torch.float32, device=device)
         ws = _lib.workspace(lib.gh_global_norm_workspace_bytes(n), device)
-        pointers = ctypes.c_void_p * n
+        ins = array("Q", map(Tensor.data_ptr, src))
+        outs = None if dst is None else ins if dst is src else array("Q", map(Tensor.data_ptr, dst))
+        sizes = array("q", map(Tensor.numel, src))
         st = lib.gh_clip_by_global_norm(
-            pointers(*[t.data_ptr() for t in src]),
-            None if dst is None else pointers(*[t.data_ptr() for t in dst]),
-            (ctypes.c_int64 * n)(*[t.numel() for t in src]),
-            (ctypes.c_int * n)(*[_lib.DTYPE_CODE[t.dtype] for t in src]),
-            n, float(max_norm), int(norm_type == math.inf), norm.data_ptr(), ws.data_ptr(), ws.numel(),
-            torch.cuda.current_stream(device).cuda_stream,
+            ins.buffer_info()[0], None if outs is None else outs.buffer_info()[0], sizes.buffer_info()[0],
+            codes.buffer_info()[0], n, float(max_norm), int(norm_type == math.inf), norm.data_ptr(), ws.data_ptr(),
+            ws.numel(), _lib.stream_handle(device),
         )
         _lib.check(st, "clip_by_global_norm")
-        if outputs is not None and dst is not None:
-            for o, d in zip(outputs, dst):
-                if d is not o:
-                    o.copy_(d)
+        for o, d in back:
+            o.detach().copy_(d)
     return norm

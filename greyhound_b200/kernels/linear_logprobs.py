@@ -90,7 +90,7 @@ def linear_logprobs(
     V = weight.shape[0]
     dev = inputs.device
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax")
         out = torch.empty(N, dtype=torch.float32, device=dev)
         lse2 = torch.empty(N, dtype=torch.float32, device=dev) if want_lse else None
@@ -104,7 +104,7 @@ def linear_logprobs(
             x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), N, D, V,
             _lib.dtype_code(x.dtype), int(ignore_index), 1.0 / float(temperature), chunk, out.data_ptr(),
             _lib.ptr(lse2), _lib.ptr(kept), 0 if kept is None else kept.numel(), ws.data_ptr(), ws.numel(),
-            _lib.stream_of(x),
+            _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax")
         _lib.raise_on_status(ws, "linear_selective_log_softmax")
@@ -131,7 +131,7 @@ def linear_logprobs_backward_kept(
     V = weight.shape[0]
     dev = inputs.device
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax backward")
         x, w, g = _operand(inputs), _operand(weight), _check_grad(grad, inputs)
         gi = torch.empty((N, D), dtype=inputs.dtype, device=dev) if want_input else None
@@ -141,7 +141,7 @@ def linear_logprobs_backward_kept(
         ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, N, 1, 1), dev)
         st = lib.gh_lsm_bwd_kept(
             x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), 1.0 / float(temperature),
-            kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(), _lib.stream_of(x),
+            kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax backward")
         _lib.raise_on_status(ws, "linear_selective_log_softmax backward")
@@ -170,7 +170,7 @@ def linear_logprobs_backward(
         if t.shape != (N,) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
             raise ValueError(f"expected {name} as a contiguous fp32 tensor of shape {(N,)} on {dev}")
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax backward")
         x, w, idx, g = _operand(inputs), _operand(weight), index.contiguous(), _check_grad(grad, inputs)
         gi = torch.empty((N, D), dtype=inputs.dtype, device=dev) if want_input else None
@@ -183,7 +183,7 @@ def linear_logprobs_backward(
             x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), logprobs.data_ptr(),
             lse2.data_ptr(), g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), int(ignore_index),
             1.0 / float(temperature), chunk, int(fp32_grad_weight_accum), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(),
-            ws.numel(), _lib.stream_of(x),
+            ws.numel(), _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax backward")
         _lib.raise_on_status(ws, "linear_selective_log_softmax backward")

@@ -20,7 +20,7 @@ __all__ = [
     "policy_loss_backward",
     "preference_loss_forward",
     "preference_loss_backward",
-    "policy_workspace_bytes",
+    "policy_state_size",
 ]
 
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
@@ -85,9 +85,18 @@ def _others(logprobs: Tensor, *ts: Tensor | None) -> tuple[int, list[Tensor | No
     return _lib.dtype_code(dtype), [None if t is None else t.to(dtype).contiguous() for t in ts]
 
 
-def policy_workspace_bytes(logprobs: Tensor, cu_seqlens: Tensor | None, reduction: str) -> int:
-    seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None else logprobs.shape[0] if logprobs.ndim == 2 else 1
-    return max(int(_lib.load().gh_policy_loss_workspace_bytes(logprobs.numel(), seqs, REDUCTIONS[reduction])), 256)
+def _seqs(logprobs: Tensor, cu_seqlens: Tensor | None) -> int:
+    return cu_seqlens.numel() - 1 if cu_seqlens is not None else logprobs.shape[0] if logprobs.ndim == 2 else 1
+
+
+def _policy_workspace(tokens: int, seqs: int, reduction: str) -> int:
+    """Floats of the policy loss's workspace, rounded to 16 bytes."""
+    return (int(_lib.load().gh_policy_loss_workspace_bytes(tokens, seqs, REDUCTIONS[reduction])) + 15) // 16 * 4
+
+
+def policy_state_size(logprobs: Tensor, cu_seqlens: Tensor | None, reduction: str, want_grad: bool) -> int:
+    tokens = logprobs.numel()
+    return 4 + _policy_workspace(tokens, _seqs(logprobs, cu_seqlens), reduction) + (tokens if want_grad else 0)
 
 
 def _advantages(advantages: Tensor, logprobs: Tensor, lay: _Layout, per: str) -> tuple[Tensor, int]:
@@ -127,12 +136,12 @@ def policy_loss_forward(
     reduction: str,
     advantages_per: str = "auto",
     want_grad: bool = True,
-) -> tuple[Tensor, Tensor, Tensor | None, Tensor]:
-    """``(loss, stats, dlogprobs or None, workspace)``.
+) -> tuple[Tensor, Tensor]:
+    """``(loss, state)``, both fp32.
 
-    ``stats`` (fp32): mean KL estimate, share of clipped tokens, valid tokens,
-    weight of a token. ``dlogprobs`` (fp32, unweighted), ``stats`` and the
-    workspace are what ``policy_loss_backward`` needs.
+    ``state`` is what ``policy_loss_backward`` needs, in one buffer: mean KL
+    estimate, share of clipped tokens, valid tokens and the weight of a token
+    (4), the workspace, and with ``want_grad`` the tokens' unweighted gradients.
     """
     if reduction not in REDUCTIONS:
         raise ValueError(f"Unsupported reduction: {reduction}")
@@ -153,29 +162,27 @@ def policy_loss_forward(
     dev = logprobs.device
     red = REDUCTIONS[reduction]
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "clipped_policy_loss")
         lp = logprobs.contiguous()
         m = None if mask is None else mask.contiguous()
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        stats = torch.empty(4, dtype=torch.float32, device=dev)
-        d = torch.empty(lay.tokens, dtype=torch.float32, device=dev) if want_grad else None
-        ws = _lib.workspace(lib.gh_policy_loss_workspace_bytes(lay.tokens, lay.seqs, red), dev)
+        ws = _policy_workspace(lay.tokens, lay.seqs, reduction)
+        state = torch.empty(4 + ws + (lay.tokens if want_grad else 0), dtype=torch.float32, device=dev)
+        at = state.data_ptr()
         st = lib.gh_policy_loss_fwd(
             lp.data_ptr(), _lib.dtype_code(lp.dtype), _lib.ptr(old), _lib.ptr(ref), other, adv.data_ptr(), per,
             _lib.ptr(m), lay.tokens, _lib.ptr(lay.cu), lay.cu_code, lay.seqs, float(clip_low), float(clip_high),
-            float(kl_multiplier), red, loss.data_ptr(), stats.data_ptr(), _lib.ptr(d), stats.data_ptr() + 12,
-            ws.data_ptr(), ws.numel(), _lib.stream_of(lp),
+            float(kl_multiplier), red, loss.data_ptr(), at, at + 16 + 4 * ws if want_grad else None, at + 12,
+            at + 16, 4 * ws, _lib.stream_handle(dev),
         )
         _lib.check(st, "clipped_policy_loss")
         _lib.raise_on_report(dev, "clipped_policy_loss")
-    return loss, stats, d, ws
+    return loss, state
 
 
 def policy_loss_backward(
-    dlogprobs: Tensor,
-    stats: Tensor,
-    workspace: Tensor,
+    state: Tensor,
     cu_seqlens: Tensor | None,
     grad_output: Tensor,
     shape: list[int] | torch.Size,
@@ -183,18 +190,21 @@ def policy_loss_backward(
     reduction: str,
 ) -> Tensor:
     """``grad_output * dloss/dlogprobs`` in ``shape`` and ``dtype``."""
-    dev = dlogprobs.device
-    tokens = dlogprobs.numel()
+    dev = state.device
+    tokens = math.prod(shape)
     seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None else shape[0] if len(shape) == 2 else 1
+    ws = _policy_workspace(tokens, seqs, reduction)
+    if state.numel() != 4 + ws + tokens:
+        raise ValueError("the state does not belong to a forward of this shape with gradients")
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "clipped_policy_loss backward")
         grad = torch.empty(shape, dtype=dtype, device=dev)
         g = grad_output.to(torch.float32)
+        at = state.data_ptr()
         st = lib.gh_policy_loss_bwd(
-            dlogprobs.data_ptr(), stats.data_ptr() + 12, workspace.data_ptr(), workspace.numel(), g.data_ptr(),
-            tokens, _lib.ptr(cu_seqlens), 0 if cu_seqlens is None else _lib.dtype_code(cu_seqlens.dtype), seqs,
-            REDUCTIONS[reduction], grad.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(dlogprobs),
+            at + 16 + 4 * ws, at + 12, at + 16, 4 * ws, g.data_ptr(), tokens, _lib.ptr(cu_seqlens), 0 if cu_seqlens is None else _lib.dtype_code(cu_seqlens.dtype), seqs,
+            REDUCTIONS[reduction], grad.data_ptr(), _lib.dtype_code(dtype), _lib.stream_handle(dev),
         )
         _lib.check(st, "clipped_policy_loss backward")
     return grad
@@ -211,8 +221,8 @@ def preference_loss_forward(
     margin: float,
     length_normalized: bool,
     reduction: str,
-) -> tuple[Tensor, Tensor, Tensor]:
-    """``(loss, rewards [sequences], gradient of a valid token [sequences])``, all fp32."""
+) -> tuple[Tensor, Tensor]:
+    """``(loss, state [2, sequences])``, fp32: rewards, and the gradient of a valid token of each sequence."""
     if reduction not in ("mean", "sum"):
         raise ValueError(f"Unsupported reduction: {reduction}")
     if loss_type not in KINDS:
@@ -236,27 +246,26 @@ def preference_loss_forward(
     other, (ref,) = _others(logprobs, ref_logprobs)
     dev = logprobs.device
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "preference_loss")
         lp = logprobs.contiguous()
         m = None if mask is None else mask.contiguous()
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        rewards = torch.empty(lay.seqs, dtype=torch.float32, device=dev)
-        coef = torch.empty(lay.seqs, dtype=torch.float32, device=dev)
+        state = torch.empty(2, lay.seqs, dtype=torch.float32, device=dev)
+        at = state.data_ptr()
         ws = _lib.workspace(lib.gh_preference_loss_workspace_bytes(lay.tokens, lay.seqs), dev)
         st = lib.gh_preference_loss_fwd(
             lp.data_ptr(), _lib.dtype_code(lp.dtype), _lib.ptr(ref), other, _lib.ptr(m), lay.tokens,
             _lib.ptr(lay.cu), lay.cu_code, lay.seqs, float(beta), float(margin), float(label_smoothing),
-            KINDS[loss_type], int(length_normalized), int(reduction == "mean"), loss.data_ptr(), rewards.data_ptr(),
-            coef.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(lp),
+            KINDS[loss_type], int(length_normalized), int(reduction == "mean"), loss.data_ptr(), at, at + 4 * lay.seqs, ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
         )
         _lib.check(st, "preference_loss")
         _lib.raise_on_report(dev, "preference_loss")
-    return loss, rewards, coef
+    return loss, state
 
 
 def preference_loss_backward(
-    coef: Tensor,
+    state: Tensor,
     grad_output: Tensor,
     mask: Tensor | None,
     cu_seqlens: Tensor | None,
@@ -264,18 +273,19 @@ def preference_loss_backward(
     dtype: torch.dtype,
 ) -> Tensor:
     """``grad_output * dloss/dlogprobs`` in ``shape`` and ``dtype``."""
-    dev = coef.device
+    dev = state.device
+    seqs = state.shape[1]
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.raise_pending(dev, "preference_loss backward")
         grad = torch.empty(shape, dtype=dtype, device=dev)
         g = grad_output.to(torch.float32)
         m = None if mask is None else mask.contiguous()
         cu = None if cu_seqlens is None else cu_seqlens.contiguous()
         st = lib.gh_preference_loss_bwd(
-            coef.data_ptr(), g.data_ptr(), _lib.ptr(m), grad.numel(), _lib.ptr(cu),
-            0 if cu is None else _lib.dtype_code(cu.dtype), coef.numel(), grad.data_ptr(), _lib.dtype_code(dtype),
-            _lib.stream_of(grad),
+            state.data_ptr() + 4 * seqs, g.data_ptr(), _lib.ptr(m), grad.numel(), _lib.ptr(cu),
+            0 if cu is None else _lib.dtype_code(cu.dtype), seqs, grad.data_ptr(), _lib.dtype_code(dtype),
+            _lib.stream_handle(dev),
         )
         _lib.check(st, "preference_loss backward")
     return grad

@@ -270,13 +270,14 @@ def clipped_policy_loss(
     alone; with ``return_metrics`` also ``PolicyLossMetrics``.
     """
     _no_grad_to(old_logprobs=old_logprobs, advantages=advantages, ref_logprobs=ref_logprobs)
-    loss, stats = ClippedPolicyLossFunction.apply(
-        logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, float(clip_low), float(clip_high),
-        float(kl_multiplier), reduction, advantages_per,
+    loss, state = ClippedPolicyLossFunction.apply(
+        logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens,
+        (float(clip_low), float(clip_high), float(kl_multiplier), reduction, advantages_per),
     )
     if not return_metrics:
         return cast(Tensor, loss)
-    return loss, PolicyLossMetrics(stats[0], stats[1], stats[2])
+    # a copy: the state holds a value per token, which kept metrics should not
+    return loss, PolicyLossMetrics(*state[:3].clone().unbind())
 
 
 def preference_loss(
@@ -313,11 +314,12 @@ def preference_loss(
     alone; with ``return_rewards`` also ``PreferenceRewards``.
     """
     _no_grad_to(ref_logprobs=ref_logprobs)
-    loss, rewards = PreferenceLossFunction.apply(
-        logprobs, ref_logprobs, mask, cu_seqlens, float(beta), loss_type, float(label_smoothing), float(margin),
-        bool(length_normalized), reduction,
+    loss, state = PreferenceLossFunction.apply(
+        logprobs, ref_logprobs, mask, cu_seqlens,
+        (float(beta), loss_type, float(label_smoothing), float(margin), bool(length_normalized), reduction),
     )
     if not return_rewards:
         return cast(Tensor, loss)
+    rewards = state[0]
     pairs = rewards.shape[0] // 2
     return loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])

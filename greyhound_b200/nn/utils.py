@@ -31,7 +31,7 @@ def global_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
     fp16, bf16 or fp32, on one device, mixed as they come; a tensor listed
     twice counts twice. Squares are summed in fp64.
     """
-    ts = [t.detach() for t in tensors]
+    ts = list(tensors)
     if not ts:
         return torch.zeros((), dtype=torch.float32, device=_device(ts))
     return clip_tensors(ts, None, 0.0, float(norm_type), _device(ts))
@@ -52,16 +52,11 @@ def clip_by_global_norm(
     tensor's input (``ValueError``). A NaN norm makes every element NaN, an
     infinite one makes finite elements 0, as the formula says.
     """
-    ts = [t.detach() for t in tensors]
-    given = None if out is None else [t.detach() for t in out]
-    # the same tensor given for both is clipped in place
-    if given is not None and len(given) == len(ts):
-        given = [
-            t if o.data_ptr() == t.data_ptr() and o.shape == t.shape and o.stride() == t.stride()
-            and o.dtype == t.dtype else o
-            for o, t in zip(given, ts)
-        ]
-    outs = [torch.empty_like(t) for t in ts] if given is None else given
+    ts = list(tensors)
+    if out is None:
+        outs = [torch.empty_like(t, requires_grad=False) for t in ts]
+    else:
+        outs = list(out)
     if not ts:
         if outs:
             raise ValueError(f"expected 0 outputs, got {len(outs)}")
@@ -86,7 +81,7 @@ def clip_grad_norm_(
     """
     if isinstance(parameters, Tensor):
         parameters = [parameters]
-    grads = [p.grad.detach() for p in parameters if p.grad is not None]
+    grads = [g for p in parameters if (g := p.grad) is not None]
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=_device(grads))
     if not float(max_norm) >= 0.0:

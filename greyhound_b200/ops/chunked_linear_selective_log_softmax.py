@@ -14,6 +14,7 @@ from typing import Any
 import torch
 from torch import Tensor
 
+from greyhound_b200 import _lib
 from greyhound_b200.kernels.linear_logprobs import (
     keeps_exponentials,
     kept_bytes,
@@ -145,15 +146,24 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
         temperature: float = 1.0,
         fp32_grad_weight_accum: bool = True,
     ) -> Tensor:
+        plain = _lib.eager(inputs) and _lib.eager(weight)
         if not ctx.needs_input_grad[0] and not ctx.needs_input_grad[1]:
+            if plain:
+                return linear_logprobs(inputs, weight, index, ignore_index, temperature)[0]
             return linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)[0]
         ctx.temperature = temperature
         ctx.kept = keeps_exponentials(inputs, weight)
         if ctx.kept:
-            out, kept = linear_selective_log_softmax_kept(inputs, weight, index, ignore_index, temperature)
+            if plain:
+                out, _, kept = linear_logprobs(inputs, weight, index, ignore_index, temperature, keep=True)
+            else:
+                out, kept = linear_selective_log_softmax_kept(inputs, weight, index, ignore_index, temperature)
             ctx.save_for_backward(inputs, weight, kept)
             return out
-        out, lse2 = linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)
+        if plain:
+            out, lse2, _ = linear_logprobs(inputs, weight, index, ignore_index, temperature, want_lse=True)
+        else:
+            out, lse2 = linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)
         ctx.ignore_index, ctx.fp32_accum = ignore_index, fp32_grad_weight_accum
         ctx.save_for_backward(inputs, weight, index, out, lse2)
         return out
@@ -164,12 +174,14 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
         want = ctx.needs_input_grad
         if ctx.kept:
             inputs, weight, kept = ctx.saved_tensors
-            gi, gw = linear_selective_log_softmax_kept_bwd(
+            bwd = linear_logprobs_backward_kept if _lib.eager(grad) else linear_selective_log_softmax_kept_bwd
+            gi, gw = bwd(
                 inputs, weight, kept, grad, ctx.temperature, want[0], want[1]
             )
         else:
             inputs, weight, index, out, lse2 = ctx.saved_tensors
-            gi, gw = linear_selective_log_softmax_bwd(
+            bwd = linear_logprobs_backward if _lib.eager(grad) else linear_selective_log_softmax_bwd
+            gi, gw = bwd(
                 inputs, weight, index, out, lse2, grad, ctx.ignore_index, ctx.temperature, ctx.fp32_accum,
                 want[0], want[1],
             )

@@ -12,10 +12,11 @@ from typing import Any
 import torch
 from torch import Tensor
 
+from greyhound_b200 import _lib
 from greyhound_b200.kernels.token_losses import (
     policy_loss_backward,
     policy_loss_forward,
-    policy_workspace_bytes,
+    policy_state_size,
     preference_loss_backward,
     preference_loss_forward,
 )
@@ -48,44 +49,36 @@ def clipped_policy_loss_fwd(
     reduction: str,
     advantages_per: str,
     want_grad: bool,
-) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    """(loss, stats [4], unweighted token gradients (empty if not wanted), workspace)."""
-    loss, stats, d, ws = policy_loss_forward(
+) -> tuple[Tensor, Tensor]:
+    """(loss, state: mean KL, clipped share, valid tokens, and what the backward reads)."""
+    return policy_loss_forward(
         logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, clip_low, clip_high, kl_multiplier,
         reduction, advantages_per, want_grad,
     )
-    return loss, stats, stats.new_empty(0) if d is None else d, ws
 
 
 @clipped_policy_loss_fwd.register_fake
 def _(logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, clip_low, clip_high, kl_multiplier,
       reduction, advantages_per, want_grad):
-    dev = logprobs.device
-    return (
-        _scalar(logprobs),
-        torch.empty([4], dtype=torch.float32, device=dev),
-        torch.empty([logprobs.numel() if want_grad else 0], dtype=torch.float32, device=dev),
-        torch.empty(policy_workspace_bytes(logprobs, cu_seqlens, reduction), dtype=torch.uint8, device=dev),
-    )
+    size = policy_state_size(logprobs, cu_seqlens, reduction, want_grad)
+    return _scalar(logprobs), torch.empty([size], dtype=torch.float32, device=logprobs.device)
 
 
 @torch.library.custom_op("greyhound::clipped_policy_loss_bwd", mutates_args=())
 def clipped_policy_loss_bwd(
-    dlogprobs: Tensor,
-    stats: Tensor,
-    workspace: Tensor,
+    state: Tensor,
     cu_seqlens: Tensor | None,
     grad_output: Tensor,
     shape: list[int],
     dtype: torch.dtype,
     reduction: str,
 ) -> Tensor:
-    return policy_loss_backward(dlogprobs, stats, workspace, cu_seqlens, grad_output, shape, dtype, reduction)
+    return policy_loss_backward(state, cu_seqlens, grad_output, shape, dtype, reduction)
 
 
 @clipped_policy_loss_bwd.register_fake
-def _(dlogprobs, stats, workspace, cu_seqlens, grad_output, shape, dtype, reduction):
-    return torch.empty(shape, dtype=dtype, device=dlogprobs.device)
+def _(state, cu_seqlens, grad_output, shape, dtype, reduction):
+    return torch.empty(shape, dtype=dtype, device=state.device)
 
 
 class ClippedPolicyLossFunction(torch.autograd.Function):
@@ -98,29 +91,23 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         ref_logprobs: Tensor | None,
         mask: Tensor | None,
         cu_seqlens: Tensor | None,
-        clip_low: float,
-        clip_high: float,
-        kl_multiplier: float,
-        reduction: str,
-        advantages_per: str,
+        options: tuple[float, float, float, str, str],  # the ops' arguments from clip_low to advantages_per
     ) -> tuple[Tensor, Tensor]:
-        loss, stats, d, ws = clipped_policy_loss_fwd(
-            logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, clip_low, clip_high, kl_multiplier,
-            reduction, advantages_per, ctx.needs_input_grad[0],
-        )
-        if ctx.needs_input_grad[0]:
-            cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-            ctx.save_for_backward(d, stats, ws, cu)
-            ctx.shape, ctx.dtype, ctx.reduction = list(logprobs.shape), logprobs.dtype, reduction
-        ctx.mark_non_differentiable(stats)
-        return loss, stats
+        want = ctx.needs_input_grad[0]
+        fwd = policy_loss_forward if _lib.eager(logprobs) else clipped_policy_loss_fwd
+        loss, state = fwd(logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, *options, want)
+        if want:
+            ctx.save_for_backward(state, None if cu_seqlens is None else cu_seqlens.contiguous())
+            ctx.like = list(logprobs.shape), logprobs.dtype, options[3]
+        ctx.mark_non_differentiable(state)
+        return loss, state
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_output: Tensor, _: Tensor):  # type: ignore[override]
-        d, stats, ws, cu = ctx.saved_tensors
-        grad = clipped_policy_loss_bwd(d, stats, ws, cu, grad_output, ctx.shape, ctx.dtype, ctx.reduction)
-        return grad, None, None, None, None, None, None, None, None, None, None
+        state, cu = ctx.saved_tensors
+        bwd = policy_loss_backward if _lib.eager(state) else clipped_policy_loss_bwd
+        return bwd(state, cu, grad_output, *ctx.like), None, None, None, None, None, None
 
 
 @torch.library.custom_op("greyhound::preference_loss_fwd", mutates_args=())
@@ -135,8 +122,8 @@ def preference_loss_fwd(
     margin: float,
     length_normalized: bool,
     reduction: str,
-) -> tuple[Tensor, Tensor, Tensor]:
-    """(loss, rewards [sequences], gradient of a valid token [sequences])."""
+) -> tuple[Tensor, Tensor]:
+    """(loss, state [2, sequences]: rewards, gradient of a valid token of each sequence)."""
     return preference_loss_forward(
         logprobs, ref_logprobs, mask, cu_seqlens, beta, loss_type, label_smoothing, margin, length_normalized,
         reduction,
@@ -147,25 +134,24 @@ def preference_loss_fwd(
 def _(logprobs, ref_logprobs, mask, cu_seqlens, beta, loss_type, label_smoothing, margin, length_normalized,
       reduction):
     seqs = cu_seqlens.shape[0] - 1 if cu_seqlens is not None else logprobs.shape[0]
-    per = [torch.empty([seqs], dtype=torch.float32, device=logprobs.device) for _ in range(2)]
-    return _scalar(logprobs), per[0], per[1]
+    return _scalar(logprobs), torch.empty([2, seqs], dtype=torch.float32, device=logprobs.device)
 
 
 @torch.library.custom_op("greyhound::preference_loss_bwd", mutates_args=())
 def preference_loss_bwd(
-    coef: Tensor,
+    state: Tensor,
     grad_output: Tensor,
     mask: Tensor | None,
     cu_seqlens: Tensor | None,
     shape: list[int],
     dtype: torch.dtype,
 ) -> Tensor:
-    return preference_loss_backward(coef, grad_output, mask, cu_seqlens, shape, dtype)
+    return preference_loss_backward(state, grad_output, mask, cu_seqlens, shape, dtype)
 
 
 @preference_loss_bwd.register_fake
-def _(coef, grad_output, mask, cu_seqlens, shape, dtype):
-    return torch.empty(shape, dtype=dtype, device=coef.device)
+def _(state, grad_output, mask, cu_seqlens, shape, dtype):
+    return torch.empty(shape, dtype=dtype, device=state.device)
 
 
 class PreferenceLossFunction(torch.autograd.Function):
@@ -176,26 +162,19 @@ class PreferenceLossFunction(torch.autograd.Function):
         ref_logprobs: Tensor | None,
         mask: Tensor | None,
         cu_seqlens: Tensor | None,
-        beta: float,
-        loss_type: str,
-        label_smoothing: float,
-        margin: float,
-        length_normalized: bool,
-        reduction: str,
+        options: tuple[float, str, float, float, bool, str],  # the ops' arguments from beta on
     ) -> tuple[Tensor, Tensor]:
-        loss, rewards, coef = preference_loss_fwd(
-            logprobs, ref_logprobs, mask, cu_seqlens, beta, loss_type, label_smoothing, margin, length_normalized,
-            reduction,
-        )
+        fwd = preference_loss_forward if _lib.eager(logprobs) else preference_loss_fwd
+        loss, state = fwd(logprobs, ref_logprobs, mask, cu_seqlens, *options)
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(coef, mask, cu_seqlens)
-            ctx.shape, ctx.dtype = list(logprobs.shape), logprobs.dtype
-        ctx.mark_non_differentiable(rewards)
-        return loss, rewards
+            ctx.save_for_backward(state, mask, cu_seqlens)
+            ctx.like = list(logprobs.shape), logprobs.dtype
+        ctx.mark_non_differentiable(state)
+        return loss, state
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_output: Tensor, _: Tensor):  # type: ignore[override]
-        coef, mask, cu = ctx.saved_tensors
-        grad = preference_loss_bwd(coef, grad_output, mask, cu, ctx.shape, ctx.dtype)
-        return grad, None, None, None, None, None, None, None, None, None
+        state, mask, cu = ctx.saved_tensors
+        bwd = preference_loss_backward if _lib.eager(state) else preference_loss_bwd
+        return bwd(state, grad_output, mask, cu, *ctx.like), None, None, None, None

@@ -264,8 +264,8 @@ def test_opcheck_compile_and_repeat():
     args = (b["lp"], b["old"], b["adv"], b["ref"], b["mask"], b["cu"], 0.2, 0.2, 0.1, "mean", "auto", True)
     # the workspace's padding is not written: no comparison of its bytes
     opcheck(clipped_policy_loss_fwd, args, test_utils=["test_schema", "test_faketensor"])
-    loss, stats, d, ws = clipped_policy_loss_fwd(*args)
-    opcheck(clipped_policy_loss_bwd, (d, stats, ws, b["cu"], loss, list(b["lp"].shape), torch.float32, "mean"))
+    loss, state = clipped_policy_loss_fwd(*args)
+    opcheck(clipped_policy_loss_bwd, (state, b["cu"], loss, list(b["lp"].shape), torch.float32, "mean"))
 
     @torch.compile(fullgraph=True)
     def f(lp):

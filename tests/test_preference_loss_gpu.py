@@ -176,8 +176,8 @@ def test_opcheck_compile_and_layouts():
     b = batch([40, 25], torch.float32, 11, True)
     args = (b["lp"], b["ref"], b["mask"], None, 0.1, "sigmoid", 0.0, 0.0, False, "mean")
     opcheck(preference_loss_fwd, args)
-    loss, rewards, coef = preference_loss_fwd(*args)
-    opcheck(preference_loss_bwd, (coef, loss, b["mask"], None, list(b["lp"].shape), torch.float32))
+    loss, state = preference_loss_fwd(*args)
+    opcheck(preference_loss_bwd, (state, loss, b["mask"], None, list(b["lp"].shape), torch.float32))
 
     @torch.compile(fullgraph=True)
     def f(lp):
