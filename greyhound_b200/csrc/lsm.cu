@@ -49,6 +49,91 @@ lsm_targets_kernel(const I* __restrict__ index, int64_t rows, int64_t V, int64_t
   tgt[r] = skip ? -1 : bad ? -2 : (int)t;
 }
 
+// Logits and statistics of one or two rows: reading W once is all the time, so
+// no tensor core and no 256-column tiles (501 of them on 148 SMs are 3.4 waves).
+// A warp takes four vocabulary rows at a time, 8 elements of each a lane and
+// step, the rows of H in shared memory as fp32; products and sums are fp32.
+// Each block leaves one (max, sum) pair a row of H. The whole call at 128256 x
+// 4096: 162 us for one row (1.05 GB at 6.5 TB/s) and 189 for two, where the GEMM
+// takes 205; at four rows shared memory and conversions made it 226. Two blocks
+// an SM with four steps of loads in flight beat more blocks with fewer.
+constexpr int kFewRows = 2;
+constexpr int kFewThreads = 256;
+constexpr int kFewSmem = 160 * 1024;
+
+template <typename T, int NR>
+__global__ void __launch_bounds__(kFewThreads, 2)
+lsm_few_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const int* __restrict__ tgt, int rows, int D,
+                    int64_t V, float sc2, float2* __restrict__ stats, float* __restrict__ xt) {
+  extern __shared__ __align__(16) float hs[];  // [NR][D]
+  __shared__ float2 part[kFewThreads / 32][NR];
+  constexpr int R = 4;
+  for (int i = threadIdx.x; i < NR * D; i += kFewThreads) hs[i] = i < rows * D ? Elt<T>::to_f(H[i]) : 0.f;
+  int t[NR];
+#pragma unroll
+  for (int k = 0; k < NR; ++k) t[k] = k < rows ? tgt[k] : -1;
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // an even share of consecutive rows: 36 or 37 of 128256, where taking groups of
+  // four in turn gives some warps 40 and the rest nothing to do meanwhile
+  const int64_t warps = (int64_t)gridDim.x * (kFewThreads / 32), me = (int64_t)blockIdx.x * (kFewThreads / 32) + warp;
+  const int64_t v1 = (me + 1) * V / warps;
+  MS ms[NR];
+#pragma unroll
+  for (int k = 0; k < NR; ++k) ms[k] = ms_empty();
+  for (int64_t v0 = me * V / warps; v0 < v1; v0 += R) {
+    const int nr = v1 - v0 < R ? (int)(v1 - v0) : R;
+    const T* w = W + v0 * D;
+    float acc[R][NR];
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+      for (int k = 0; k < NR; ++k) acc[j][k] = 0.f;
+#pragma unroll 4
+    for (int d = lane * 8; d < D; d += 256) {
+      Vec16<T> x[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j)  // past the last row: the first one again, not used
+        x[j].raw = ld16_last(w + (int64_t)(j < nr ? j : 0) * D + d);
+      float f[R][8];
+#pragma unroll
+      for (int j = 0; j < R; ++j) x[j].to_float(f[j]);
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        const float4 a = *reinterpret_cast<const float4*>(hs + k * D + d);
+        const float4 b = *reinterpret_cast<const float4*>(hs + k * D + d + 4);
+        const float h[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int j = 0; j < R; ++j) acc[j][k] = fmaf(f[j][e], h[e], acc[j][k]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        float s = acc[j][k];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (j >= nr) continue;
+        if (t[k] == v0 + j && lane == 0) xt[k] = s;
+        // a NaN logit has to stay in the sum
+        ms[k] = s == s ? ms_fold1(ms[k], s * sc2) : MS{0.f, s};
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NR; ++k)
+    if (lane == 0) part[warp][k] = make_float2(ms[k].m, ms[k].s);
+  __syncthreads();
+  if (threadIdx.x < rows) {
+    MS a = ms_empty();
+    for (int i = 0; i < kFewThreads / 32; ++i) a = ms_merge(a, MS{part[i][threadIdx.x].x, part[i][threadIdx.x].y});
+    stats[(int64_t)blockIdx.x * rows + threadIdx.x] = make_float2(a.m, a.s);
+  }
+}
+
 struct CombineOut {
   float* y;        // [rows] log-probability of the target (0: left out)
   float* lse2;     // [rows] log-sum-exp, log2 units (may be NULL)
@@ -344,7 +429,9 @@ FwdLayout fwd_layout(int64_t N, int64_t V, int64_t chunk, bool keep) {
   L.xt = off;      off = al256(off + sizeof(float) * chunk);
   L.lse2 = off;    off = al256(off + sizeof(float) * N);
   L.rowflag = off; off = al256(off + sizeof(int) * (keep ? N : 0));
-  L.stats = off;   off = al256(off + sizeof(float2) * (size_t)L.num_n * chunk);
+  // the kernel for few rows leaves one pair a block, at most 8 blocks an SM
+  const size_t parts = N <= kFewRows && L.num_n < 8 * num_sms_dev() ? 8 * num_sms_dev() : L.num_n;
+  L.stats = off;   off = al256(off + sizeof(float2) * parts * chunk);
   L.qmode = off;   off = al256(off + (keep ? (size_t)L.num_n * 2 * chunk : 0));
   L.gmax = off;    off = al256(off + (keep ? sizeof(float) * (size_t)L.num_n * 2 * chunk : 0));
   L.total = off;
@@ -423,6 +510,35 @@ int logits_gemm(const void* H, const void* W, int64_t rows, int64_t D, int64_t V
   return launch_gemm_t<T, 0, 0, EPI, T, 1>(ta, tb, p, num_sms_dev(), st);
 }
 
+// Blocks of lsm_few_rows_kernel, or 0 where the GEMM runs.
+template <typename T, int NR>
+int few_rows_blocks(int64_t D, int64_t V) {
+  const size_t smem = (size_t)NR * D * sizeof(float);
+  if (smem > kFewSmem) return 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  auto kern = lsm_few_rows_kernel<T, NR>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) != cudaSuccess) return 0;
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kFewThreads, smem) != cudaSuccess || per_sm < 1)
+    return 0;
+  const int64_t most = (V + 4 * (kFewThreads / 32) - 1) / (4 * (kFewThreads / 32));
+  const int64_t blocks = (int64_t)per_sm * num_sms_dev();
+  return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T, int NR>
+int few_rows(const void* H, const void* W, const int* tgt, int64_t rows, int64_t D, int64_t V, float sc2,
+             float2* stats, int* blocks, float* xt, cudaStream_t st) {
+  *blocks = few_rows_blocks<T, NR>(D, V);
+  if (!*blocks) return GH_OK;
+  ProfScope prof(PROF_GEMM_LOGITS_CE, st);
+  lsm_few_rows_kernel<T, NR><<<*blocks, kFewThreads, (size_t)NR * D * sizeof(float), st>>>(
+      static_cast<const T*>(H), static_cast<const T*>(W), tgt, (int)rows, (int)D, V, sc2, stats, xt);
+  count_launch(1);
+  return check_launch("lsm_few_rows");
+}
+
 int check_common(int64_t N, int64_t D, int64_t V, int dtype, int index_dtype, double inv_t) {
   if (dtype != GH_BF16 && dtype != GH_F16)
     return set_error(GH_ETYPE, "expected bf16 or fp16 operands (dtype code %d)", dtype);
@@ -472,12 +588,21 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
         if ((rc = logits_gemm<T, gemm::EPI_LSM_Q>(Hc, W, rows, D, V, dtype, p, st))) return rc;
       }
     }
-    if (!kept && (rc = logits_gemm<T, gemm::EPI_LSM>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+    int parts = L.num_n;
+    if (!kept) {
+      int few = 0;
+      if (N <= kFewRows) {
+        if (N == 1) rc = few_rows<T, 1>(Hc, W, tgt, rows, D, V, sc2, stats, &few, xt, st);
+        else rc = few_rows<T, kFewRows>(Hc, W, tgt, rows, D, V, sc2, stats, &few, xt, st);
+        if (rc) return rc;
+      }
+      if (few) parts = few;
+      else if ((rc = logits_gemm<T, gemm::EPI_LSM>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+    }
     if (rows <= 4 * (int64_t)num_sms_dev())
-      lsm_combine_kernel<1><<<(unsigned)rows, 256, 0, st>>>(stats, L.num_n, rows, V, sc2, xt, tgt + s0, o);
+      lsm_combine_kernel<1><<<(unsigned)rows, 256, 0, st>>>(stats, parts, rows, V, sc2, xt, tgt + s0, o);
     else
-      lsm_combine_kernel<32><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(stats, L.num_n, rows, V, sc2, xt, tgt + s0,
-                                                                          o);
+      lsm_combine_kernel<32><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(stats, parts, rows, V, sc2, xt, tgt + s0, o);
     count_launch(1);
     if ((rc = check_launch("lsm_combine"))) return rc;
     if (kept) {

@@ -212,6 +212,34 @@ def test_scoring_and_training_forwards_agree_in_every_bit(monkeypatch, scale):
 
 
 @requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("D,V", [(8, 1), (8, 9), (264, 3), (72, 257), (1032, 4099), (4096, 20_003), (12_296, 1000), (40_968, 65)])
+def test_scoring_few_rows(N, D, V, dtype):
+    """One or two rows without a gradient have a kernel of their own, while they fit shared memory."""
+    H, W, t, g = make(N, D, V, dtype, N + D, scale=3.0, left_out=0.3)
+    for temperature in (1.0, 0.6):
+        y = chunked_linear_selective_log_softmax(H, W, t, temperature=temperature)
+        ry, _, _, ey, _, _ = definition(H, W, t, g, temperature)
+        assert ((y.double() - ry).abs() <= ey).all()
+        assert (y[t == -100] == 0).all()
+
+
+@requires_gpu
+def test_scoring_few_rows_with_odd_values():
+    H, W, t, g = make(2, 64, 500, torch.bfloat16, 30, left_out=0.0)
+    clean = chunked_linear_selective_log_softmax(H, W, t)
+    H[1, 5] = float("nan")
+    y = chunked_linear_selective_log_softmax(H, W, t)
+    assert y[1].isnan() and y[0] == clean[0]
+    t[1] = -100
+    assert chunked_linear_selective_log_softmax(H, W, t)[1] == 0
+    H[1] = 0.0
+    W[7, 0] = float("nan")  # one logit of each row
+    assert chunked_linear_selective_log_softmax(H, W, t)[0].isnan()
+
+
+@requires_gpu
 def test_retained_graph_takes_other_gradients():
     H, W, t, g = make(150, 128, 1000, torch.bfloat16, 12)
     h, w = H.requires_grad_(True), W.requires_grad_(True)
