@@ -190,21 +190,22 @@ def policy_loss_backward(
     reduction: str,
 ) -> Tensor:
     """``grad_output * dloss/dlogprobs`` in ``shape`` and ``dtype``."""
+    # runs on autograd's thread, where every line costs more than in the forward
     dev = state.device
     tokens = math.prod(shape)
     seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None else shape[0] if len(shape) == 2 else 1
-    ws = _policy_workspace(tokens, seqs, reduction)
-    if state.numel() != 4 + ws + tokens:
+    ws = state.numel() - 4 - tokens
+    if ws < 0:
         raise ValueError("the state does not belong to a forward of this shape with gradients")
-    lib = _lib.load()
     with _lib.on_device(dev):
         _lib.raise_pending(dev, "clipped_policy_loss backward")
         grad = torch.empty(shape, dtype=dtype, device=dev)
-        g = grad_output.to(torch.float32)
+        g = grad_output if grad_output.dtype == torch.float32 else grad_output.to(torch.float32)
         at = state.data_ptr()
-        st = lib.gh_policy_loss_bwd(
-            at + 16 + 4 * ws, at + 12, at + 16, 4 * ws, g.data_ptr(), tokens, _lib.ptr(cu_seqlens), 0 if cu_seqlens is None else _lib.dtype_code(cu_seqlens.dtype), seqs,
-            REDUCTIONS[reduction], grad.data_ptr(), _lib.dtype_code(dtype), _lib.stream_handle(dev),
+        st = _lib.load().gh_policy_loss_bwd(
+            at + 16 + 4 * ws, at + 12, at + 16, 4 * ws, g.data_ptr(), tokens, _lib.ptr(cu_seqlens),
+            0 if cu_seqlens is None else _lib.DTYPE_CODE[cu_seqlens.dtype], seqs, REDUCTIONS[reduction],
+            grad.data_ptr(), _lib.DTYPE_CODE[dtype], _lib.stream_handle(dev),
         )
         _lib.check(st, "clipped_policy_loss backward")
     return grad

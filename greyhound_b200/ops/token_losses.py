@@ -100,11 +100,14 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
             ctx.save_for_backward(state, None if cu_seqlens is None else cu_seqlens.contiguous())
             ctx.like = list(logprobs.shape), logprobs.dtype, options[3]
         ctx.mark_non_differentiable(state)
+        ctx.set_materialize_grads(False)  # no zeros for state's gradient, which nobody reads
         return loss, state
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_output: Tensor, _: Tensor):  # type: ignore[override]
+        if grad_output is None:
+            return (None,) * 7
         state, cu = ctx.saved_tensors
         bwd = policy_loss_backward if _lib.eager(state) else clipped_policy_loss_bwd
         return bwd(state, cu, grad_output, *ctx.like), None, None, None, None, None, None
@@ -170,11 +173,14 @@ class PreferenceLossFunction(torch.autograd.Function):
             ctx.save_for_backward(state, mask, cu_seqlens)
             ctx.like = list(logprobs.shape), logprobs.dtype
         ctx.mark_non_differentiable(state)
+        ctx.set_materialize_grads(False)  # no zeros for state's gradient, which nobody reads
         return loss, state
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_output: Tensor, _: Tensor):  # type: ignore[override]
+        if grad_output is None:
+            return (None,) * 5
         state, mask, cu = ctx.saved_tensors
         bwd = preference_loss_backward if _lib.eager(state) else preference_loss_bwd
         return bwd(state, grad_output, mask, cu, *ctx.like), None, None, None, None
