@@ -36,17 +36,33 @@ constexpr double kLog2ed = 1.4426950408889634;
 // Row kernels
 
 // Clean targets: -1 for a row that is left out, -2 for an index outside
-// [0, V) (flagged; its log-probability is NaN and it has no gradient).
+// [0, V) (flagged; its log-probability is NaN and it has no gradient). One block
+// also clears the status word first; more blocks find it cleared.
 template <typename I>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 lsm_targets_kernel(const I* __restrict__ index, int64_t rows, int64_t V, int64_t ignore, int* __restrict__ tgt,
                    int* status) {
-  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (r >= rows) return;
-  const int64_t t = (int64_t)index[r];
-  const bool skip = t == ignore, bad = !skip && (t < 0 || t >= V);
-  if (bad) atomicOr(status, GH_DEV_BAD_LABEL);
-  tgt[r] = skip ? -1 : bad ? -2 : (int)t;
+  if (gridDim.x == 1) {
+    if (threadIdx.x == 0) *status = 0;
+    __syncthreads();
+  }
+  for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows; r += (int64_t)gridDim.x * 1024) {
+    const int64_t t = (int64_t)index[r];
+    const bool skip = t == ignore, bad = !skip && (t < 0 || t >= V);
+    if (bad) atomicOr(status, GH_DEV_BAD_LABEL);
+    tgt[r] = skip ? -1 : bad ? -2 : (int)t;
+  }
+}
+
+// The last kernel of a call hands its status on to the device's sticky slot.
+__device__ __forceinline__ void publish(const int* status, int* slot) {
+  if (slot && blockIdx.x == 0 && threadIdx.x == 0) {
+    const int v = *reinterpret_cast<const volatile int*>(status);
+    if (v) {
+      volatile int* h = slot;
+      *h = *h | v;
+    }
+  }
 }
 
 // Logits and statistics of one or two rows: reading W once is all the time, so
@@ -141,9 +157,32 @@ struct CombineOut {
   __nv_bfloat16* q;
   int64_t ldq;
   const uint8_t* qmode;
+  const float* gmax;
   float* alpha0;   // [rows] factor that turns the stored row into p - onehot; 0: left out
-  int* rowflag;    // [rows] 1: rewrite the row, 2: zero it
+  const int* status;
+  int* slot;       // not NULL in a call's last launch
 };
+
+// Rewrite a row that q cannot represent (a group outside the exponent window,
+// a log-sum-exp outside it) as p - onehot, or zero one that is left out and
+// whose values are no fit operand; by a whole block.
+__device__ __forceinline__ void lsm_fix_row(const CombineOut& o, int64_t rows, int64_t row, int64_t V, int flag,
+                                            float l2, float y, int t) {
+  __nv_bfloat16* q = o.q + row * o.ldq;
+  for (int64_t c = threadIdx.x; c < V; c += blockDim.x) {
+    float v = 0.f;
+    if (flag == 1) {
+      const int64_t grp = ((c >> 8) * 2 + ((c >> 7) & 1)) * rows + row;
+      const float stored = __bfloat162float(q[c]);
+      const float up = (o.qmode[grp] ? o.gmax[grp] : 0.f) - l2;
+      // 2^up alone may overflow or vanish where the product does not
+      v = stored > 0.f ? fast_exp2(fast_log2(stored) + up) : stored;
+      if (up != up) v = up;  // a log-sum-exp of NaN: the row's gradient is NaN
+      if (c == t) v = expm1f(y);
+    }
+    q[c] = __float2bfloat16_rn(v);
+  }
+}
 
 // Merge the per-tile (max, sum) pairs of TR rows per block. TR = 32 reads
 // 32 rows x 8 tiles at a time (coalesced: the partials are [tile][row]); few
@@ -185,60 +224,41 @@ lsm_combine_kernel(const float2* __restrict__ stats, int num_n, int64_t rows, in
     }
     __syncthreads();
   }
-  if (slice != 0 || r >= rows) return;
-  const double lse2 = (double)sm[tid] + log2((double)ss[tid]);
-  const int t = tgt[r];
-  double y = t >= 0 ? kLn2d * ((double)xt[r] * (double)sc2 - lse2) : 0.0;
-  if (y > 0.0) y = 0.0;  // rounding at p = 1; a NaN stays
-  o.y[r] = t == -2 ? __int_as_float(0x7fc00000) : (float)y;
-  if (o.lse2) o.lse2[r] = (float)lse2;
-  if (!o.q) return;
-  const bool odd = sf[tid] || !(lse2 >= (double)gemm::kLsmQLo && lse2 <= (double)gemm::kLsmQHi + 32.0);
-  if (t < 0) {
-    // a left-out row must not reach the gradients, not even as 0 * NaN
-    o.alpha0[r] = 0.f;
-    o.rowflag[r] = odd ? 2 : 0;
-    return;
-  }
-  // The target's entry of p - onehot is -(1 - p_t) = expm1(y); it outweighs
-  // its row. Its 16-bit rounding would reach dW on top of the one of a * H, so
-  // the row factor takes it out: alpha0 * (stored target) is exact to fp32, and
-  // the row's other entries, each rounded already, move by at most 2^-9.
-  const double tau = expm1(y) * (odd ? 1.0 : exp2(lse2));
-  const __nv_bfloat16 c = __float2bfloat16_rn((float)tau);
-  const double cd = (double)__bfloat162float(c);
-  const double fix = cd != 0.0 ? tau / cd : 1.0;
-  o.alpha0[r] = (float)((odd ? 1.0 : exp2(-lse2)) * fix);
-  o.rowflag[r] = odd ? 1 : 0;
-  if (!odd) o.q[r * o.ldq + t] = c;
-}
-
-// Rewrite the rows that q cannot represent (a group outside the exponent
-// window, a log-sum-exp outside it) as p - onehot, and zero left-out rows
-// whose values are no fit operand. Most rows return at once.
-__global__ void __launch_bounds__(256)
-lsm_fixup_kernel(__nv_bfloat16* q, int64_t ld, const uint8_t* __restrict__ qmode, const float* __restrict__ gmax,
-                 const int* __restrict__ rowflag, const float* __restrict__ lse2, const float* __restrict__ y,
-                 const int* __restrict__ tgt, int64_t rows, int64_t V) {
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int f = rowflag[row];
-    if (!f) continue;
-    __nv_bfloat16* yq = q + row * ld;
-    const int t = tgt[row];
-    const float l2 = lse2[row];
-    for (int64_t c = threadIdx.x; c < V; c += 256) {
-      float v = 0.f;
-      if (f == 1) {
-        const int64_t grp = ((c >> 8) * 2 + ((c >> 7) & 1)) * rows + row;
-        const float stored = __bfloat162float(yq[c]);
-        const float up = (qmode[grp] ? gmax[grp] : 0.f) - l2;
-        // 2^up alone may overflow or vanish where the product does not
-        v = stored > 0.f ? fast_exp2(fast_log2(stored) + up) : stored;
-        if (up != up) v = up;  // a log-sum-exp of NaN: the row's gradient is NaN
-        if (c == t) v = expm1f(y[row]);
+  if (slice == 0 && r < rows) {
+    const double lse2 = (double)sm[tid] + log2((double)ss[tid]);
+    const int t = tgt[r];
+    double y = t >= 0 ? kLn2d * ((double)xt[r] * (double)sc2 - lse2) : 0.0;
+    if (y > 0.0) y = 0.0;  // rounding at p = 1; a NaN stays
+    o.y[r] = t == -2 ? __int_as_float(0x7fc00000) : (float)y;
+    if (o.lse2) o.lse2[r] = (float)lse2;
+    if (o.q) {
+      const bool odd = sf[tid] || !(lse2 >= (double)gemm::kLsmQLo && lse2 <= (double)gemm::kLsmQHi + 32.0);
+      sf[tid] = !odd ? 0 : t >= 0 ? 1 : 2;
+      sm[tid] = (float)lse2;
+      ss[tid] = (float)y;
+      if (t < 0) {
+        o.alpha0[r] = 0.f;  // must not reach the gradients, not even as 0 * NaN
+      } else {
+        // The target's entry of p - onehot is -(1 - p_t) = expm1(y); it outweighs
+        // its row. Its 16-bit rounding would reach dW on top of the one of a * H,
+        // so the row factor takes it out: alpha0 * (stored target) is exact to
+        // fp32, and the row's other entries, each rounded already, move by at
+        // most 2^-9.
+        const double tau = expm1(y) * (odd ? 1.0 : exp2(lse2));
+        const __nv_bfloat16 c = __float2bfloat16_rn((float)tau);
+        const double cd = (double)__bfloat162float(c);
+        const double fix = cd != 0.0 ? tau / cd : 1.0;
+        o.alpha0[r] = (float)((odd ? 1.0 : exp2(-lse2)) * fix);
+        if (!odd) o.q[r * o.ldq + t] = c;
       }
-      yq[c] = __float2bfloat16_rn(v);
     }
+  }
+  publish(o.status, o.slot);
+  if (!o.q) return;
+  __syncthreads();
+  for (int i = 0; i < TR; ++i) {
+    const int64_t row = (int64_t)blockIdx.x * TR + i;
+    if (row < rows && sf[i]) lsm_fix_row(o, rows, row, V, sf[i], sm[i], ss[i], tgt[row]);
   }
 }
 
@@ -247,7 +267,9 @@ lsm_fixup_kernel(__nv_bfloat16* q, int64_t ld, const uint8_t* __restrict__ qmode
 // the output's). Left-out rows give exact zeros.
 __global__ void __launch_bounds__(256)
 lsm_rows_kernel(const __nv_bfloat16* __restrict__ H, const float* __restrict__ g, const float* __restrict__ alpha0,
-                float inv_t, int64_t rows, int64_t D, float* __restrict__ a_out, __nv_bfloat16* __restrict__ hs) {
+                float inv_t, int64_t rows, int64_t D, float* __restrict__ a_out, __nv_bfloat16* __restrict__ hs,
+                int* status) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;  // for the GEMMs that follow
   const int64_t vpr = D / 8, n = rows * vpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / vpr;
@@ -321,7 +343,8 @@ lsm_clean_rows_kernel(const uint4* __restrict__ H, const int* __restrict__ tgt, 
 template <typename T>
 __global__ void __launch_bounds__(256)
 lsm_join_kernel(const float* __restrict__ part, int slices, int64_t n, int64_t D, const float* __restrict__ row,
-                const float* __restrict__ scale, T* __restrict__ out) {
+                const float* __restrict__ scale, T* __restrict__ out, const int* status, int* slot) {
+  publish(status, slot);
   const float f = scale ? *scale : 1.f;
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     float4 a = *reinterpret_cast<const float4*>(part + i);
@@ -376,10 +399,11 @@ size_t dh_scratch(int64_t rows, int64_t D, int64_t V) {
   return (size_t)rows * D * (s ? (size_t)s * 4 : 2);
 }
 
-// dH[rows, D] = row[r] * scale * (A[rows, V] W[V, D]).
+// dH[rows, D] = row[r] * scale * (A[rows, V] W[V, D]). Where slices are joined,
+// the join hands the status on to `slot`.
 template <typename T>
 int dh_gemm(int dtype, const Operand& A, const void* W, int64_t rows, int64_t D, int64_t V, void* out,
-            const float* scale, const float* row, void* scratch, int* status, cudaStream_t st) {
+            const float* scale, const float* row, void* scratch, int* status, int* slot, cudaStream_t st) {
   const int slices = dh_slices(rows, D, V);
   const int sms = num_sms_dev();
   const Operand B{W, D, 1};
@@ -407,13 +431,14 @@ int dh_gemm(int dtype, const Operand& A, const void* W, int64_t rows, int64_t D,
   }
   const int64_t n = rows * D, want = (n + 1023) / 1024, cap = 8 * (int64_t)sms;
   lsm_join_kernel<T><<<(unsigned)(want < cap ? want : cap), 256, 0, st>>>(static_cast<const float*>(scratch), slices, n,
-                                                                        D, row, scale, static_cast<T*>(out));
+                                                                        D, row, scale, static_cast<T*>(out), status,
+                                                                        slot);
   count_launch(1);
   return check_launch("lsm_join");
 }
 
 struct FwdLayout {
-  size_t status = 0, tgt, xt, lse2, rowflag, stats, qmode, gmax, total;
+  size_t status = 0, tgt, xt, lse2, stats, qmode, gmax, total;
   int64_t chunk;
   int num_n;
 };
@@ -428,7 +453,6 @@ FwdLayout fwd_layout(int64_t N, int64_t V, int64_t chunk, bool keep) {
   L.tgt = off;     off = al256(off + sizeof(int) * N);
   L.xt = off;      off = al256(off + sizeof(float) * chunk);
   L.lse2 = off;    off = al256(off + sizeof(float) * N);
-  L.rowflag = off; off = al256(off + sizeof(int) * (keep ? N : 0));
   // the kernel for few rows leaves one pair a block, at most 8 blocks an SM
   const size_t parts = N <= kFewRows && L.num_n < 8 * num_sms_dev() ? 8 * num_sms_dev() : L.num_n;
   L.stats = off;   off = al256(off + sizeof(float2) * parts * chunk);
@@ -482,11 +506,12 @@ BwdLayout bwd_layout(int64_t N, int64_t D, int64_t V, int64_t chunk, bool kept, 
 
 int targets(const void* index, int index_dtype, int64_t N, int64_t V, int64_t ignore, int* tgt, int* status,
             cudaStream_t st) {
-  const unsigned grid = (unsigned)((N + 255) / 256);
+  const unsigned grid = N <= 16384 ? 1 : (unsigned)((N + 1023) / 1024);
+  if (grid > 1) cudaMemsetAsync(status, 0, sizeof(int), st);
   if (index_dtype == GH_I64)
-    lsm_targets_kernel<int64_t><<<grid, 256, 0, st>>>(static_cast<const int64_t*>(index), N, V, ignore, tgt, status);
+    lsm_targets_kernel<int64_t><<<grid, 1024, 0, st>>>(static_cast<const int64_t*>(index), N, V, ignore, tgt, status);
   else
-    lsm_targets_kernel<int32_t><<<grid, 256, 0, st>>>(static_cast<const int32_t*>(index), N, V, ignore, tgt, status);
+    lsm_targets_kernel<int32_t><<<grid, 1024, 0, st>>>(static_cast<const int32_t*>(index), N, V, ignore, tgt, status);
   count_launch(1);
   return check_launch("lsm_targets");
 }
@@ -560,7 +585,9 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
   float* xt = reinterpret_cast<float*>(ws + L.xt);
   float2* stats = reinterpret_cast<float2*>(ws + L.stats);
   const KeptLayout K = kept_layout(N, V);
-  int rc;
+  int* slot = nullptr;
+  int rc = device_error_slot(&slot);
+  if (rc) return rc;
   for (int64_t s0 = 0; s0 < N; s0 += L.chunk) {
     const int64_t rows = s0 + L.chunk <= N ? L.chunk : N - s0;
     gemm::Params p{};
@@ -572,6 +599,8 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
     CombineOut o{};
     o.y = y + s0;
     o.lse2 = lse2 + s0;
+    o.status = status;
+    o.slot = s0 + rows >= N ? slot : nullptr;
     const void* Hc = static_cast<const T*>(H) + s0 * D;
     if constexpr (sizeof(T) == 2 && gemm::AbType<T>::v == 1) {
       if (kept) {
@@ -583,8 +612,8 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
         o.q = reinterpret_cast<__nv_bfloat16*>(kept + K.q);
         o.ldq = K.ldq;
         o.qmode = p.qmode;
+        o.gmax = p.gmax;
         o.alpha0 = reinterpret_cast<float*>(kept + K.alpha0);
-        o.rowflag = reinterpret_cast<int*>(ws + L.rowflag);
         if ((rc = logits_gemm<T, gemm::EPI_LSM_Q>(Hc, W, rows, D, V, dtype, p, st))) return rc;
       }
     }
@@ -605,15 +634,8 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
       lsm_combine_kernel<32><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(stats, parts, rows, V, sc2, xt, tgt + s0, o);
     count_launch(1);
     if ((rc = check_launch("lsm_combine"))) return rc;
-    if (kept) {
-      const int64_t cap = 8 * (int64_t)num_sms_dev();
-      lsm_fixup_kernel<<<(unsigned)(rows < cap ? rows : cap), 256, 0, st>>>(o.q, o.ldq, o.qmode, p.gmax, o.rowflag,
-                                                                           o.lse2, o.y, tgt, rows, V);
-      count_launch(1);
-      if ((rc = check_launch("lsm_fixup"))) return rc;
-    }
   }
-  return publish_status(status, st);
+  return GH_OK;
 }
 
 int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V, float inv_t,
@@ -621,21 +643,24 @@ int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N,
   int* status = reinterpret_cast<int*>(ws + L.status);
   const KeptLayout K = kept_layout(N, V);
   const int sms = num_sms_dev();
+  int* slot = nullptr;
+  int rc = device_error_slot(&slot);
+  if (rc) return rc;
   float* a = reinterpret_cast<float*>(ws + L.rfac);
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(ws + L.hs);
   lsm_rows_kernel<<<4 * sms, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(H), grad,
                                            reinterpret_cast<const float*>(kept + K.alpha0), inv_t, N, D, a,
-                                           dW ? hs : nullptr);
+                                           dW ? hs : nullptr, status);
   count_launch(1);
-  int rc = check_launch("lsm_rows");
-  if (rc) return rc;
+  if ((rc = check_launch("lsm_rows"))) return rc;
   if (dW && (rc = run_gemm(GH_BF16, Operand{kept + K.q, K.ldq, 1}, Operand{hs, D, 1}, V, D, N, dW, GH_BF16, D, nullptr,
                            nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
     return rc;
   if (dH && (rc = dh_gemm<__nv_bfloat16>(GH_BF16, Operand{kept + K.q, K.ldq, 0}, W, N, D, V, dH, nullptr, a,
-                                         ws + L.dh2, status, st)))
+                                         ws + L.dh2, status, slot, st)))
     return rc;
-  return publish_status(status, st);
+  // a joined dH has published in its last launch
+  return dH && dh_slices(N, D, V) ? GH_OK : publish_status(status, st);
 }
 
 template <typename T>
@@ -698,7 +723,7 @@ int lsm_bwd_run(const void* H, const void* W, const float* y, const float* lse2,
         return rc;
     }
     if (dH && (rc = dh_gemm<T>(dtype, Operand{d, L.ldd, 0}, W, rows, D, V, static_cast<T*>(dH) + s0 * D, unscale,
-                               nullptr, ws + L.dh2, status, st)))
+                               nullptr, ws + L.dh2, status, nullptr, st)))
       return rc;
   }
   return publish_status(status, st);
@@ -739,7 +764,6 @@ extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int i
   char* ws = static_cast<char*>(workspace);
   const float sc2 = (float)(inv_temperature * kLog2ed);
   int* status = reinterpret_cast<int*>(ws + L.status);
-  cudaMemsetAsync(status, 0, sizeof(int), st);
   if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
   char* kp = static_cast<char*>(kept);
   if (dtype == GH_BF16) return lsm_fwd_run<__nv_bfloat16>(H, W, N, D, V, dtype, sc2, L, kp, logprobs, lse2, ws, st);
@@ -761,7 +785,6 @@ extern "C" int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, 
     return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  cudaMemsetAsync(ws + L.status, 0, sizeof(int), st);
   return lsm_bwd_kept_run(H, W, grad, N, D, V, (float)inv_temperature, static_cast<const char*>(kept), grad_input,
                           grad_weight, L, ws, st);
 }
@@ -784,7 +807,6 @@ extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int i
   const float inv_t = (float)inv_temperature;
   const float sc2 = (float)(inv_temperature * kLog2ed);
   int* status = reinterpret_cast<int*>(ws + L.status);
-  cudaMemsetAsync(status, 0, sizeof(int), st);
   if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
   if (dtype == GH_BF16)
     return lsm_bwd_run<__nv_bfloat16>(H, W, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, grad_input, grad_weight,
