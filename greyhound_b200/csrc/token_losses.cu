@@ -16,10 +16,11 @@
 // latency below. Up to kOneBlock tokens one block does the whole forward in
 // one launch.
 //
-// A term is fp32; differences of log-probabilities, sums and what decides
-// between a clip's two sides are fp64 (the losses cancel: a mean of 1e-3 over
-// terms of size 1 would keep only 4 digits of an fp32 sum, and the fp64 adds
-// hide behind the loads).
+// A policy term is fp32, and so is the sum of the four that a lane has at hand;
+// what goes on from there is fp64 (the loss cancels: a mean of 1e-3 over a
+// million terms of size 1 would keep few digits of an fp32 sum). A ratio within
+// 2^-16 of a clip bound is decided in fp64. The preference sums are fp64 from the
+// first difference on: they decide a whole sequence's gradient.
 #include <cmath>
 
 #include "common.cuh"
@@ -146,6 +147,7 @@ struct Policy {
   int adv_per_seq;
   const uint8_t* mask;
   double lo, hi;       // log(1 - el), log(1 + eh)
+  float lo_f, hi_f;    // the same, rounded
   float at_lo, at_hi;  // 1 - el, 1 + eh
   float k;
   float* d;            // [T] gradient of l_t; NULL: not wanted
@@ -161,11 +163,12 @@ struct PolicyOut {
   Sums *warps, *slots, *seqs;
 };
 
-// e^u - 1 - u without the cancellation at small u: the Taylor series there
-// (|u| < 1/4: the next term is below 2^-24 of the sum).
-__device__ __forceinline__ float expm1_minus(float u, float em1) {
-  if (fabsf(u) >= 0.25f) return em1 - u;
-  float p = 1.f / 362880.f;
+// e^u - 1 and e^u - 1 - u. Differences of e^u would cancel at small u: the second
+// comes from its Taylor series there (|u| < 1/2: the next term is below 2^-28 of
+// the sum) and the first is u plus it.
+__device__ __forceinline__ float kl_terms(float u, float& em1) {
+  float p = 1.f / 3628800.f;
+  p = fmaf(p, u, 1.f / 362880.f);
   p = fmaf(p, u, 1.f / 40320.f);
   p = fmaf(p, u, 1.f / 5040.f);
   p = fmaf(p, u, 1.f / 720.f);
@@ -173,7 +176,11 @@ __device__ __forceinline__ float expm1_minus(float u, float em1) {
   p = fmaf(p, u, 1.f / 24.f);
   p = fmaf(p, u, 1.f / 6.f);
   p = fmaf(p, u, 0.5f);
-  return u * u * p;
+  const float near = u * u * p;
+  const bool small = fabsf(u) < 0.5f;
+  const float far = expf(u) - 1.f;
+  em1 = small ? u + near : far;
+  return small ? near : far - u;
 }
 
 // The warp's tokens [t0, t1): gradients, one Sums per part (want_slots) and
@@ -194,62 +201,79 @@ __device__ __forceinline__ void policy_tokens(const Seqs& q, const Policy& p, in
       return;
     }
     Sums sum{0.0, 0.0, 0, 0};
-    const float adv_s = p.adv_per_seq ? p.adv[s] : 0.f;
+    // 32-bit offsets from the part's first token (a part is at most a span).
+    // What is absent is read with stride 0 from an address that is there: no
+    // branch stands between a lane's loads, and none of them waits for the mask.
+    const int n = (int)(b - a);
+    const T* lpa = lp + a;
+    const R* olda = p.old ? old + a : reinterpret_cast<const R*>(p.adv);
+    const R* refa = KL ? ref + a : nullptr;
+    const float* adva = p.adv_per_seq ? p.adv + s : p.adv + a;
+    const uint8_t* maska = p.mask ? p.mask + a : reinterpret_cast<const uint8_t*>(p.adv);
+    const int olds = p.old ? 1 : 0, advs = p.adv_per_seq ? 0 : 1, masks = p.mask ? 1 : 0;
+    float* da = p.d ? p.d + a : nullptr;
     constexpr int U = 4;
-    for (int64_t t = a + lane; t < b; t += 32 * U) {
+    for (int t = lane; t < n; t += 32 * U) {
       bool on[U];
       float x[U], y[U], z[U], av[U];
+      T xr[U];
+      R yr[U], zr[U];
+      uint8_t mr[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t i = t + 32 * j;
-        on[j] = i < b && (!p.mask || p.mask[i]);
+        const int i = t + 32 * j < n ? t + 32 * j : t;  // past the end: the lane's first token again
+        mr[j] = maska[i * masks];
+        xr[j] = lpa[i];
+        yr[j] = olda[i * olds];
+        if (KL) zr[j] = refa[i];
+        av[j] = adva[i * advs];
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t i = t + 32 * j;
-        x[j] = y[j] = z[j] = 0.f;
-        av[j] = adv_s;
-        // not only where the mask is set: that would wait for the mask first
-        // (21 against 16 us for 2 million positions, 44 % of them left out)
-        if (i < b) {
-          x[j] = Elt<T>::to_f(lp[i]);
-          y[j] = p.old ? Elt<R>::to_f(old[i]) : x[j];
-          if (KL) z[j] = Elt<R>::to_f(ref[i]);
-          if (!p.adv_per_seq) av[j] = p.adv[i];
-        }
+        on[j] = t + 32 * j < n && (!masks || mr[j]);
+        x[j] = Elt<T>::to_f(xr[j]);
+        y[j] = olds ? Elt<R>::to_f(yr[j]) : x[j];
+        z[j] = KL ? Elt<R>::to_f(zr[j]) : 0.f;
       }
+      float l4 = 0.f, k4 = 0.f;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t i = t + 32 * j;
         float g = 0.f;
         if (on[j]) {
           const float A = av[j];
-          const double d = (double)x[j] - (double)y[j];
-          const bool above = A > 0.f && d > p.hi, below = A < 0.f && d < p.lo;
+          const float d = x[j] - y[j];
+          bool above = d > p.hi_f, below = d < p.lo_f;
+          if (fabsf(d - p.hi_f) < 0x1p-16f || fabsf(d - p.lo_f) < 0x1p-16f) {
+            const double e = (double)x[j] - (double)y[j];
+            above = e > p.hi;
+            below = e < p.lo;
+          }
+          above = above && A > 0.f;
+          below = below && A < 0.f;
           float l;
           if (above || below) {
             l = -A * (above ? p.at_hi : p.at_lo);
           } else {
-            l = -A * expf((float)d);
+            l = -A * expf(d);
             g = l;
           }
-          double lt = l;
           if (KL) {
-            const float u = (float)((double)z[j] - (double)x[j]);
-            const float em1 = expm1f(u);
-            const float k3 = expm1_minus(u, em1);
+            float em1;
+            const float k3 = kl_terms(z[j] - x[j], em1);
             if (p.k != 0.f) {  // 0 times an infinite term is no term
               g = fmaf(-p.k, em1, g);
-              lt += (double)p.k * k3;
+              l = fmaf(p.k, k3, l);
             }
-            sum.kl += k3;
+            k4 += k3;
           }
-          sum.loss += lt;
+          l4 += l;
           sum.clipped += above || below;
           sum.n += 1;
         }
-        if (p.d && i < b) p.d[i] = g;
+        if (da && t + 32 * j < n) da[t + 32 * j] = g;
       }
+      sum.loss += (double)l4;
+      if (KL) sum.kl += (double)k4;
     }
     sum.loss = warp_sum(sum.loss);
     if (KL) sum.kl = warp_sum(sum.kl);
@@ -359,10 +383,18 @@ policy_bwd_kernel(Seqs q, const float* __restrict__ d, const float* __restrict__
   const float c = scal[0] * go[0];
   const int64_t t0 = w * span, t1 = t0 + span < q.T ? t0 + span : q.T;
   auto part = [&](float f, int64_t a, int64_t b) {
-#pragma unroll 4
-    for (int64_t t = a + lane; t < b; t += 32) {
-      const float x = d[t];
-      grad[t] = Elt<T>::from_f(x == 0.f ? 0.f : x * f);  // a token left out stays 0 under any grad_output
+    const int n = (int)(b - a);
+    const float* da = d + a;
+    T* ga = grad + a;
+    // independent loads before the first store, which may alias them for all the compiler knows
+    constexpr int U = 8;
+    for (int t = lane; t < n; t += 32 * U) {
+      float x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[j] = t + 32 * j < n ? da[t + 32 * j] : 0.f;
+#pragma unroll
+      for (int j = 0; j < U; ++j)  // a token left out stays 0 under any grad_output
+        if (t + 32 * j < n) ga[t + 32 * j] = Elt<T>::from_f(x[j] == 0.f ? 0.f : x[j] * f);
     }
   };
   if (!seqs) {
@@ -417,22 +449,23 @@ __device__ __forceinline__ void pref_tokens(const Seqs& q, const Pref& p, int64_
     if (s < 0) return;
     double sum = 0.0;
     int n = 0;
+    const int len = (int)(b - a);
+    const T* lpa = lp + a;
+    const R* refa = ref ? ref + a : nullptr;
+    const uint8_t* maska = p.mask ? p.mask + a : nullptr;
     constexpr int U = 8;
-    for (int64_t t = a + lane; t < b; t += 32 * U) {
+    for (int t = lane; t < len; t += 32 * U) {
       bool on[U];
       float x[U], y[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t i = t + 32 * j;
-        on[j] = i < b && (!p.mask || p.mask[i]);
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int64_t i = t + 32 * j;
+        const int i = t + 32 * j;
+        on[j] = i < len;
         x[j] = y[j] = 0.f;
-        if (i < b) {  // mask or not: its load need not come first
-          x[j] = Elt<T>::to_f(lp[i]);
-          if (ref) y[j] = Elt<R>::to_f(ref[i]);
+        if (i < len) {  // mask or not: its load need not come first
+          if (maska) on[j] = maska[i];
+          x[j] = Elt<T>::to_f(lpa[i]);
+          if (refa) y[j] = Elt<R>::to_f(refa[i]);
         }
       }
 #pragma unroll
@@ -544,8 +577,18 @@ pref_bwd_kernel(Seqs q, const uint8_t* __restrict__ mask, const float* __restric
   const int64_t t0 = w * span, t1 = t0 + span < q.T ? t0 + span : q.T;
   walk(q, t0, t1, [&](int64_t s, int64_t a, int64_t b) {
     const T v = Elt<T>::from_f(s >= 0 ? coef[s] * g : 0.f), zero = Elt<T>::from_f(0.f);
-#pragma unroll 8
-    for (int64_t t = a + lane; t < b; t += 32) grad[t] = !mask || mask[t] ? v : zero;
+    const int n = (int)(b - a);
+    T* ga = grad + a;
+    const uint8_t* maska = mask ? mask + a : nullptr;
+    constexpr int U = 8;
+    for (int t = lane; t < n; t += 32 * U) {
+      bool on[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) on[j] = !maska || (t + 32 * j < n && maska[t + 32 * j]);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (t + 32 * j < n) ga[t + 32 * j] = on[j] ? v : zero;
+    }
   });
 }
 
@@ -718,6 +761,8 @@ extern "C" int gh_policy_loss_fwd(const void* logprobs, int dtype, const void* o
   p.mask = mask;
   p.lo = clip_low < 1.0 ? log1p(-clip_low) : -HUGE_VAL;
   p.hi = log1p(clip_high);
+  p.lo_f = (float)p.lo;
+  p.hi_f = (float)p.hi;
   p.at_lo = (float)(1.0 - clip_low);
   p.at_hi = (float)(1.0 + clip_high);
   p.k = (float)kl_multiplier;

@@ -1,9 +1,10 @@
 """clipped_policy_loss against its formula in 64 bits.
 
-Tolerances: an fp32 term is e^d from a rounded d, with expf's 2 ulp and a few
-products: relative 2^-24 (|d| + 8), of |A| e^d, or of k (|e^u - 1| + |u|) for the
-KL term, in which e^u - 1 - u is a difference where |u| >= 1/4. Sums are fp64, results
-fp32 (2^-24) or in the log-probabilities' type (half a step each).
+Tolerances: an fp32 term is e^d from a rounded d, with expf's ulp, a product and
+up to three additions of four terms: relative 2^-24 (|d| + 8), of |A| e^d, or of
+k (|e^u - 1| + |u|) for the KL term, in which e^u - 1 - u is a difference where
+|u| >= 1/2. Further sums are fp64, results fp32 (2^-24) or in the log-probabilities'
+type (half a step each).
 """
 
 import math
