@@ -227,7 +227,8 @@ scale_kernel(const __grid_constant__ List<MAX> l, const double* __restrict__ par
   __shared__ double scratch[kThreads / 32];
   const double norm = finish((A*)nullptr, norm_of<A>(part, parts, scratch));
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) *norm_out = (float)norm;
-  const double cd = max_norm / (norm + 1e-6);
+  // no limit: nothing to scale, whatever the norm
+  const double cd = max_norm == HUGE_VAL ? 1.0 : max_norm / (norm + 1e-6);
   const float c = cd >= 1.0 ? 1.f : (float)cd;
   if (in_place && c == 1.f) return;
   const int total = l.first[l.count];

@@ -64,7 +64,8 @@ def _chunk(N: int, D: int, V: int) -> int:
 
 
 def kept_bytes(N: int, V: int) -> int:
-    return max(int(_lib.load().gh_lsm_kept_bytes(N, V)), 256)
+    """``gh_lsm_kept_bytes``, in arithmetic that symbolic sizes go through, too."""
+    return ((N * ((V + 7) // 8 * 8) * 2 + 255) // 256 + (4 * N + 255) // 256) * 256
 
 
 def keeps_exponentials(inputs: Tensor, weight: Tensor) -> bool:

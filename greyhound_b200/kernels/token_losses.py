@@ -95,8 +95,8 @@ def _policy_workspace(tokens: int, seqs: int, reduction: str) -> int:
 
 
 def policy_state_size(logprobs: Tensor, cu_seqlens: Tensor | None, reduction: str, want_grad: bool) -> int:
-    tokens = logprobs.numel()
-    return 4 + _policy_workspace(tokens, _seqs(logprobs, cu_seqlens), reduction) + (tokens if want_grad else 0)
+    tokens, seqs = int(logprobs.numel()), int(_seqs(logprobs, cu_seqlens))  # symbolic sizes become these
+    return 4 + _policy_workspace(tokens, seqs, reduction) + (tokens if want_grad else 0)
 
 
 def _advantages(advantages: Tensor, logprobs: Tensor, lay: _Layout, per: str) -> tuple[Tensor, int]:

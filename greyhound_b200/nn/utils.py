@@ -50,7 +50,8 @@ def clip_by_global_norm(
     ``tensors`` themselves for clipping in place, which writes nothing when the
     norm is below ``max_norm``. Outputs may not overlap each other or another
     tensor's input (``ValueError``). A NaN norm makes every element NaN, an
-    infinite one makes finite elements 0, as the formula says.
+    infinite one makes finite elements 0, as the formula says; an infinite
+    ``max_norm`` changes nothing.
     """
     ts = list(tensors)
     if out is None:

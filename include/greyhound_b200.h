@@ -427,8 +427,8 @@ GH_API int gh_preference_loss_bwd(const float* coef, const float* grad_output, c
  * inf_norm the largest absolute value, to *norm (device F32); and, unless
  * outputs is NULL, outputs[i] = min(1, max_norm / (norm + 1e-6)) * tensors[i] in
  * the tensor's type. outputs[i] may be tensors[i]; otherwise outputs overlap
- * neither inputs nor each other (GH_EINVAL). The arrays are read before the
- * call returns.
+ * neither inputs nor each other (GH_EINVAL). An infinite max_norm scales
+ * nothing. The arrays are read before the call returns.
  * ------------------------------------------------------------------------ */
 GH_API size_t gh_global_norm_workspace_bytes(int64_t count);
 GH_API int gh_clip_by_global_norm(const void* const* tensors, void* const* outputs, const int64_t* numels,

@@ -184,6 +184,9 @@ def test_zero_limit_and_zero_gradients():
     ts = make([(100,)], [torch.float32], 10)
     outs, _ = clip_by_global_norm(ts, 0.0)
     assert (outs[0] == 0).all()
+    ts[0][3] = math.inf
+    outs, norm = clip_by_global_norm(ts, math.inf)
+    assert norm.item() == math.inf and torch.equal(outs[0], ts[0])  # no limit, no change
     zero = [torch.zeros(1000, device="cuda")]
     outs, norm = clip_by_global_norm(zero, 1.0)
     assert norm.item() == 0.0 and (outs[0] == 0).all()

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from greyhound_b200 import _lib
+from greyhound_b200.kernels.linear_logprobs import kept_bytes
 from greyhound_b200.nn.functional import chunked_linear_selective_log_softmax as f
 
 BF = torch.bfloat16
@@ -63,6 +64,8 @@ def test_buffer_sizes():
     """Stored e^x is 2 bytes a logit; the forward without it, and the
     recomputed backward, do not grow with N * V."""
     lib = _lib.load()
+    for n, v in ((1, 1), (7, 9), (64, 100), (65, 128256), (16384, 131072)):
+        assert kept_bytes(n, v) == lib.gh_lsm_kept_bytes(n, v)
     assert lib.gh_lsm_kept_bytes(8192, 128256) < 8192 * 128256 * 2 + (1 << 20)
     assert lib.gh_lsm_fwd_workspace_bytes(65536, 128256, 8192, 0) < 64 << 20
     assert lib.gh_lsm_bwd_workspace_bytes(65536, 4096, 128256, 8192, 0, 1) < (2 << 30) + 4 * 4096 * 128256 + (256 << 20)

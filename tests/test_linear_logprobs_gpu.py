@@ -339,3 +339,43 @@ def test_deterministic_and_capturable():
     torch.cuda.synchronize()
     for a, b in zip(out, eager):
         assert torch.equal(a.detach(), b)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_compile(dtype):
+    H, W, t, g = make(60, 64, 300, dtype, 18)
+    f = torch.compile(chunked_linear_selective_log_softmax, fullgraph=True)
+    h, w = H.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    y = f(h, w, t, temperature=0.8)
+    got = torch.autograd.grad(y, (h, w), g)
+    want_y, *want = check(H, W, t, g, temperature=0.8)
+    assert torch.equal(y, want_y) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@requires_gpu
+@pytest.mark.parametrize("N,V", [(16_300, 131_072), (17_000, 131_072)])
+def test_large_products(N, V):
+    """N * V beyond 2^31 bytes, kept (4.27 GB of e^x) and, above 4 GiB, recomputed in several
+    chunks: some rows of dH and of dW against 64 bits, with the bounds above."""
+    H, W, t, g = make(N, 64, V, torch.bfloat16, 19, scale=2.0)
+    assert K.keeps_exponentials(H, W) == (N == 16_300)
+    h, w = H.requires_grad_(True), W.requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, w, t)
+    dh, dw = torch.autograd.grad(y, (h, w), g)
+    rows = torch.cat([torch.arange(0, N, 97, device="cuda"), torch.arange(N - 5, N, device="cuda")])
+    with torch.no_grad():
+        ry, rH, _, ey, bH, _ = definition(H[rows], W, t[rows], g[rows])
+        assert ((y[rows].double() - ry).abs() <= ey).all()
+        assert ((dh[rows].double() - rH).abs() <= bH).all()
+        # columns of the logits' gradient: p from all rows' log-sum-exp
+        cols = torch.cat([t[rows[:20]].clamp(min=0), torch.arange(V - 5, V, device="cuda")])
+        lse = torch.cat([torch.logsumexp(x.double() @ W.double().T, 1) for x in H.split(1024)])
+        x = H.double() @ W[cols].double().T
+        gg = torch.where(t != -100, g.double(), 0.0)[:, None]
+        p = (x - lse[:, None]).exp()
+        d = gg * ((t[:, None] == cols).double() - p)
+        u = U[torch.bfloat16]
+        rW = d.T @ H.double()
+        bW = (3 * u * d.abs() + ey * gg.abs() * p).T @ H.double().abs() + 2 * u * rW.abs()
+        assert ((dw[cols].double() - rW).abs() <= bW + 2.0**-62 * (gg.abs() * H.double().abs()).sum(0)).all()
