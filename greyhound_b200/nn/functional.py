@@ -216,18 +216,17 @@ def chunked_linear_selective_log_softmax(
     _check_accum_dtype(grad_weight_accum_dtype)
     if inputs.ndim < 1 or index.shape != inputs.shape[:-1]:
         raise ValueError(f"expected index shape {tuple(inputs.shape[:-1])}, got {tuple(index.shape)}")
-    flat = cast(
+    flat, flat_index = inputs, index
+    if inputs.ndim != 2:  # not for two dimensions: a view is a step of autograd's, both ways
+        flat = inputs.reshape(index.numel(), inputs.shape[-1])
+        flat_index = index.reshape(-1)
+    out = cast(
         Tensor,
         ChunkedLinearSelectiveLogSoftmaxFunction.apply(
-            inputs.reshape(-1, inputs.shape[-1]) if inputs.shape[-1] else inputs.reshape(index.numel(), 0),
-            weight,
-            index.reshape(-1),
-            ignore_index,
-            float(temperature),
-            grad_weight_accum_dtype == "fp32",
+            flat, weight, flat_index, ignore_index, float(temperature), grad_weight_accum_dtype == "fp32"
         ),
     )
-    return flat.reshape(index.shape)
+    return out if inputs.ndim == 2 else out.reshape(index.shape)
 
 
 def clipped_policy_loss(
