@@ -66,6 +66,14 @@ constexpr float kQLo = -80.f;
 // gradient of 2^-27 and a hidden value of 2^-7 is still a normal bf16 number.
 constexpr float kLsmQHi = 64.f;
 constexpr float kLsmQLo = -64.f;
+// The tensor core truncates its accumulator at every K = 16 step, always towards
+// zero: over K = 4096 logits of size 2 came out 9e-6 off. The log-probability
+// epilogues take the product in segments of kLsmSeg 64-wide k-steps, each with an
+// accumulator of its own, and add those up in fp32 registers. Forward at
+// 8192 x 4096 x 128256: one segment 5.36 ms and an error of 6.7e-7 of the
+// log-probabilities' size, two (32 steps each) 5.48 ms and 3e-7, four 5.64 ms and
+// 1.5e-7.
+constexpr int kLsmSeg = 32;
 
 struct Params {
   int M, N, K;
@@ -405,18 +413,6 @@ __device__ __forceinline__ void lce_fold_chunk(const uint32_t* w, int c, int n0,
   lce_target_from_chunk<OutT>(w, c, lab_rel, xt_row);
 }
 
-// One of 32 register values by a run-time index li in [0, 32), as a chain of
-// selects (an indexed load would move the array to local memory).
-__device__ __forceinline__ uint32_t select32(const uint32_t (&r)[32], int li) {
-  uint32_t v = 0;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %2, %3;\n\tselp.b32 %0, %1, %0, p;\n\t}"
-        : "+r"(v)
-        : "r"(r[j]), "r"(li), "r"(j));
-  return v;
-}
-
 // Geometry of one configuration. PAIR = 1: one CTA computes a 128 x 256 tile.
 // PAIR = 2: a 2-CTA cluster computes a 256 x 256 tile with tcgen05.mma
 // cta_group::2; each CTA stages its 128 rows of A and 128 of the 256 B rows,
@@ -649,11 +645,15 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       for (int tile = unit; tile < p.num_tiles; tile += nunits) {
         const TileK tk = tile_k(p, tile, nkb);
         const int nkt = tk.kb1 - tk.kb0;
-        if (!tc::mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, lim)) break;
+        bool ok = true;
+        // one segment, except for the log-probability epilogues
+        const int seg = EPI >= EPI_LSM ? kLsmSeg : nkt;
+        for (int k0 = 0; k0 < nkt && ok; k0 += seg) {
+        if (!tc::mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, lim)) { ok = false; break; }
         tc::tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        bool ok = true;
-        for (int kb = 0; kb < nkt; ++kb) {
+        const int k1 = k0 + seg < nkt ? k0 + seg : nkt;
+        for (int kb = k0; kb < k1; ++kb) {
           if (!tc::mbar_wait(&full[stage], phase, abort_flag, lim)) { ok = false; break; }
           tc::tc_fence_after();
           const uint32_t a0 = tc::smem_u32(sA + stage * G::A_BYTES);
@@ -662,8 +662,9 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t ad = tc::smem_desc_sw128(a0 + k * a_kstep, a_lbo, a_sbo);
             const uint64_t bd = tc::smem_desc_sw128(b0 + k * b_kstep, b_lbo, b_sbo);
-            if (PAIR == 2) tc::mma_f16_pair(d_tmem, ad, bd, idesc, (kb | k) != 0);
-            else tc::mma_f16(d_tmem, ad, bd, idesc, (kb | k) != 0);
+            const bool add = ((kb - k0) | k) != 0;
+            if (PAIR == 2) tc::mma_f16_pair(d_tmem, ad, bd, idesc, add);
+            else tc::mma_f16(d_tmem, ad, bd, idesc, add);
           }
           if (PAIR == 2) tc::mma_commit_pair_mc(&empty[stage], 0x3);
           else tc::mma_commit(&empty[stage]);
@@ -673,6 +674,8 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         if (PAIR == 2) tc::mma_commit_pair_mc(&tfull[acc], 0x3);
         else tc::mma_commit(&tfull[acc]);
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+        if (!ok) break;
       }
     }
   } else if (warp >= EPI_WARP0) {
@@ -697,7 +700,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       void* const pout = NSUB == 1 && p.split_bytes ? static_cast<char*>(p.out) + tk.ks * p.split_bytes
                          : tk.ks ? p.out2 : p.out;
       const int m0 = mt * G::TM + (int)rank * BM;
-      if (NSUB == 1) {
+      if (NSUB == 1 && EPI < EPI_LSM) {
         if (!tc::mbar_wait(&tfull[acc], acc_phase, abort_flag, lim)) break;
         tc::tc_fence_after();
       }
@@ -728,7 +731,126 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         xbuf ^= 1;
         return ok;
       };
-      if constexpr (NSUB == 2) {
+      if constexpr (EPI >= EPI_LSM) {
+        // ---- linear log-probabilities ----
+        // This row's 128 columns of the tile: the segments' accumulators are
+        // added up in registers, each freed as soon as it is read, and all else
+        // works from there.
+        constexpr int NV = EPI_CHUNKS * 32;
+        float v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = 0.f;
+        const int n0 = nt * G::TN, c0 = g * EPI_CHUNKS, col_g = n0 + c0 * 32;
+        for (int k0 = 0; k0 < tk.kb1 - tk.kb0; k0 += kLsmSeg) {
+          if (!tc::mbar_wait(&tfull[acc], acc_phase, abort_flag, lim)) { stop = true; break; }
+          tc::tc_fence_after();
+          __syncwarp();
+          const uint32_t tb = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + c0 * 32;
+#pragma unroll
+          for (int i = 0; i < NV / 16; ++i) {
+            uint32_t r[16];
+            tc::tmem_ld16_wait(tb + i * 16, r);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[i * 16 + j] += __uint_as_float(r[j]);
+          }
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR == 2) tc::mbar_arrive_cluster(acc ? tempty_leader1 : tempty_leader0);
+            else tc::mbar_arrive(&tempty[acc]);
+          }
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+        if (stop) break;
+        if constexpr (EPI == EPI_LSM_GRAD) {
+          // The logits' gradient straight from the recomputed logits:
+          // rfac (onehot - e^(x - lse)), rounded once. The target's own value
+          // comes from -expm1(log-probability): no cancellation at p near 1.
+          const int t = row_ok ? p.tgt[row] : -1;
+          const float l2 = t >= 0 ? p.lse2[row] : 0.f;
+          const float f = t >= 0 ? p.rfac[row] : 0.f;
+          const float tv = t >= 0 ? p.tval[row] : 0.f;
+#pragma unroll
+          for (int i = 0; i < EPI_CHUNKS; ++i) {
+            const int col0 = col_g + i * 32;
+            if (col0 >= p.N) break;
+            const int li = t - col0;
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float d0 = -f * fast_exp2(fmaf(v[i * 32 + 2 * j], p.sc2, -l2));
+              float d1 = -f * fast_exp2(fmaf(v[i * 32 + 2 * j + 1], p.sc2, -l2));
+              // a row without a target: 0 even where the logits are NaN
+              d0 = t < 0 ? 0.f : li == 2 * j ? tv : d0;
+              d1 = t < 0 ? 0.f : li == 2 * j + 1 ? tv : d1;
+              w[j] = pack2<OutT>(d0, d1);
+            }
+            store_chunk_packed<OutT>(reinterpret_cast<OutT*>(pout), p.ldo, m0 + q * 32, p.M, col0, p.N, w, stage_out,
+                                     lane, p.vec_ok, p.out_evict_first);
+          }
+        } else {
+          // The target's logit and, per row and 256-column tile, (max, sum of
+          // exponentials). EPI_LSM_Q also stores q = e^x in 16 bits (one ex2
+          // does both), as e^(x - shift) with the group's largest logit as the
+          // shift where that lies outside the window: two roundings of e^x
+          // relative to itself, whatever the size of the logits. Without the
+          // store the sums are formed the same way, so that a scoring pass and
+          // a training pass over the same rows agree in every bit (the ratio of
+          // their probabilities is exactly 1).
+          const int t_rel = (row_ok ? p.tgt[row] : -1) - col_g;
+          float cmax = kNegInf;
+          if (col_g + NV <= p.N) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) cmax = fmaxf(cmax, v[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+              if (col_g + j < p.N) cmax = fmaxf(cmax, v[j]);
+          }
+          const float cml = cmax * p.sc2;
+          const bool out_of_window = !(cml <= kLsmQHi && (cml >= kLsmQLo || cml == kNegInf));  // NaN: out
+          const float shift = out_of_window ? cml : 0.f;
+          if constexpr (EPI == EPI_LSM_Q) {
+            if (row_ok && col_g < p.N) {
+              const int64_t gi = ((int64_t)nt * 2 + g) * p.M + row;
+              p.qmode[gi] = out_of_window ? 1 : 0;
+              if (out_of_window) p.gmax[gi] = cml;
+            }
+          }
+          if ((unsigned)t_rel < (unsigned)NV) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) x = t_rel == j ? v[j] : x;
+            p.xt[row] = x;
+          }
+          __syncwarp();
+          float s_run = 0.f;
+#pragma unroll
+          for (int i = 0; i < EPI_CHUNKS; ++i) {
+            const int col0 = col_g + i * 32;
+            if (col0 >= p.N) break;
+            const bool full = col0 + 32 <= p.N;
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float a = fast_exp2(fmaf(v[i * 32 + 2 * j], p.sc2, -shift));
+              float b = fast_exp2(fmaf(v[i * 32 + 2 * j + 1], p.sc2, -shift));
+              if (!full) {
+                if (col0 + 2 * j >= p.N) a = 0.f;
+                if (col0 + 2 * j + 1 >= p.N) b = 0.f;
+              }
+              s_run += a + b;
+              if constexpr (EPI == EPI_LSM_Q) w[j] = pack2<OutT>(a, b);
+            }
+            if constexpr (EPI == EPI_LSM_Q)
+              store_chunk_packed<OutT>(reinterpret_cast<OutT*>(pout), p.ldo, m0 + q * 32, p.M, col0, p.N, w, stage_out,
+                                       lane, p.vec_ok, p.out_evict_first);
+          }
+          const float m_run = s_run == 0.f ? kNegInf : shift;  // a NaN sum must not look empty to the merge
+          __syncwarp();
+          if (!stats_exchange_at(0, m_run, s_run)) stop = true;
+        }
+      } else if constexpr (NSUB == 2) {
         {
           // 512-column tile, 16-bit output. Each warp drains its 4 chunks of a
           // half from TMEM, finishes the first at once and parks the other 3
@@ -892,104 +1014,6 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               s_run = s_q;
             }
             if (!stats_exchange_at(h, m_run, s_run)) stop = true;
-          } else if constexpr (EPI == EPI_LSM || EPI == EPI_LSM_Q) {
-            // Log-probability statistics from the fp32 accumulator: the
-            // target's logit and, per row and 256-column tile, (max, sum of
-            // exponentials). EPI_LSM_Q also stores q = e^x in 16 bits (one
-            // ex2 does both), as e^(x - shift) with the group's largest logit
-            // as the shift where that lies outside the window: two roundings
-            // of e^x relative to itself, whatever the size of the logits.
-            // Without the store the sums are formed the same way, so that a
-            // scoring pass and a training pass over the same rows agree in
-            // every bit (the ratio of their probabilities is exactly 1).
-            const int t_rel = (row_ok ? p.tgt[row] : -1) - n0;
-            float cmax = kNegInf;
-#pragma unroll 1
-            for (int i = 0; i < EPI_CHUNKS; ++i) {
-              uint32_t r[32];
-              tc::tmem_ld32(tbase + i * 32, r);
-              tc::tmem_ld_wait(r);
-              const int col0 = n0 + (c0 + i) * 32;
-              if (col0 + 32 <= p.N) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) cmax = fmaxf(cmax, __uint_as_float(r[j]));
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col0 + j < p.N) cmax = fmaxf(cmax, __uint_as_float(r[j]));
-              }
-            }
-            const float cml = cmax * p.sc2;
-            const bool out_of_window = !(cml <= kLsmQHi && (cml >= kLsmQLo || cml == kNegInf));  // NaN: out
-            const float shift = out_of_window ? cml : 0.f;
-            float s_run = 0.f;
-            if constexpr (EPI == EPI_LSM_Q) {
-              if (row_ok && n0 + c0 * 32 < p.N) {
-                const int64_t gi = ((int64_t)nt * 2 + g) * p.M + row;
-                p.qmode[gi] = out_of_window ? 1 : 0;
-                if (out_of_window) p.gmax[gi] = cml;
-              }
-            }
-#pragma unroll 1
-            for (int i = 0; i < EPI_CHUNKS; ++i) {
-              const int c = c0 + i;
-              const int col0 = n0 + c * 32;
-              if (col0 >= p.N) break;
-              const bool full = col0 + 32 <= p.N;
-              uint32_t r[32];
-              __syncwarp();  // the target's lane may still be in its branch
-              tc::tmem_ld32(tbase + i * 32, r);
-              tc::tmem_ld_wait(r);
-              const int li = t_rel - c * 32;
-              if ((unsigned)li < 32u) p.xt[row] = __uint_as_float(select32(r, li));
-              uint32_t w[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                float a = fast_exp2(fmaf(__uint_as_float(r[2 * j]), p.sc2, -shift));
-                float b = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), p.sc2, -shift));
-                if (!full) {
-                  if (col0 + 2 * j >= p.N) a = 0.f;
-                  if (col0 + 2 * j + 1 >= p.N) b = 0.f;
-                }
-                s_run += a + b;
-                if constexpr (EPI == EPI_LSM_Q) w[j] = pack2<OutT>(a, b);
-              }
-              if constexpr (EPI == EPI_LSM_Q)
-                store_chunk_packed<OutT>(reinterpret_cast<OutT*>(pout), p.ldo, m0 + q * 32, p.M, col0, p.N, w,
-                                         stage_out, lane, p.vec_ok, p.out_evict_first);
-            }
-            const float m_run = s_run == 0.f ? kNegInf : shift;  // a NaN sum must not look empty to the merge
-            __syncwarp();
-            if (!stats_exchange_at(h, m_run, s_run)) stop = true;
-          } else if constexpr (EPI == EPI_LSM_GRAD) {
-            // The logits' gradient straight from the recomputed accumulator:
-            // rfac (onehot - e^(x - lse)), rounded once. The target's own value
-            // comes from -expm1(log-probability): no cancellation at p near 1.
-            const int t = row_ok ? p.tgt[row] : -1;
-            const float l2 = row_ok && t >= 0 ? p.lse2[row] : 0.f;
-            const float f = row_ok && t >= 0 ? p.rfac[row] : 0.f;
-            const uint32_t tv = __float_as_uint(row_ok && t >= 0 ? p.tval[row] : 0.f);
-#pragma unroll 1
-            for (int i = 0; i < EPI_CHUNKS; ++i) {
-              const int c = c0 + i;
-              const int col0 = n0 + c * 32;
-              if (col0 >= p.N) break;
-              uint32_t r[32];
-              tc::tmem_ld32(tbase + i * 32, r);
-              tc::tmem_ld_wait(r);
-              const int li = t - col0;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float d = -f * fast_exp2(fmaf(__uint_as_float(r[j]), p.sc2, -l2));
-                r[j] = t < 0 ? 0u : li == j ? tv : __float_as_uint(d);  // a row without a target: 0 even where NaN
-              }
-              uint32_t w[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                w[j] = pack2<OutT>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-              store_chunk_packed<OutT>(reinterpret_cast<OutT*>(pout), p.ldo, m0 + q * 32, p.M, col0, p.N, w,
-                                       stage_out, lane, p.vec_ok, p.out_evict_first);
-            }
           } else if constexpr (EPI == EPI_LCE) {
             const int64_t lab = row_ok ? p.labels[row] - p.label_offset : -1;
             const int64_t lab_rel = lab - n0;  // label column inside this half, if any
