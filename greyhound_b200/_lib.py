@@ -107,8 +107,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "gh_lsm_bwd": (
         _i32,
-        [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i64, _f64, _i64, _i32, _vp, _vp, _vp, _sz,
-         _vp],
+        [_vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _i64, _f64, _i64, _i32, _vp, _vp, _vp, _sz, _vp],
     ),
     "gh_policy_loss_workspace_bytes": (_sz, [_i64, _i64, _i32]),
     "gh_policy_loss_fwd": (

@@ -153,6 +153,7 @@ lsm_few_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const int*
 struct CombineOut {
   float* y;        // [rows] log-probability of the target (0: left out)
   float* lse2;     // [rows] log-sum-exp, log2 units (may be NULL)
+  float* y2;       // [rows] y once more, for the backward (may be NULL)
   // kept form only (q == NULL otherwise)
   __nv_bfloat16* q;
   int64_t ldq;
@@ -231,6 +232,7 @@ lsm_combine_kernel(const float2* __restrict__ stats, int num_n, int64_t rows, in
     if (y > 0.0) y = 0.0;  // rounding at p = 1; a NaN stays
     o.y[r] = t == -2 ? __int_as_float(0x7fc00000) : (float)y;
     if (o.lse2) o.lse2[r] = (float)lse2;
+    if (o.y2) o.y2[r] = (float)y;
     if (o.q) {
       const bool odd = sf[tid] || !(lse2 >= (double)gemm::kLsmQLo && lse2 <= (double)gemm::kLsmQHi + 32.0);
       sf[tid] = !odd ? 0 : t >= 0 ? 1 : 2;
@@ -578,10 +580,10 @@ int check_common(int64_t N, int64_t D, int64_t V, int dtype, int index_dtype, do
 
 template <typename T>
 int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, int dtype, float sc2,
-                const FwdLayout& L, char* kept, float* y, float* lse2_out, char* ws, cudaStream_t st) {
+                const FwdLayout& L, char* kept, float* y, float* state, char* ws, cudaStream_t st) {
   int* status = reinterpret_cast<int*>(ws + L.status);
   int* tgt = reinterpret_cast<int*>(ws + L.tgt);
-  float* lse2 = lse2_out ? lse2_out : reinterpret_cast<float*>(ws + L.lse2);
+  float* lse2 = state ? state : reinterpret_cast<float*>(ws + L.lse2);
   float* xt = reinterpret_cast<float*>(ws + L.xt);
   float2* stats = reinterpret_cast<float2*>(ws + L.stats);
   const KeptLayout K = kept_layout(N, V);
@@ -599,6 +601,7 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
     CombineOut o{};
     o.y = y + s0;
     o.lse2 = lse2 + s0;
+    o.y2 = state ? state + N + s0 : nullptr;
     o.status = status;
     o.slot = s0 + rows >= N ? slot : nullptr;
     const void* Hc = static_cast<const T*>(H) + s0 * D;
@@ -749,7 +752,7 @@ extern "C" size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, in
 
 extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int index_dtype, int64_t N, int64_t D,
                           int64_t V, int dtype, int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
-                          float* logprobs, float* lse2, void* kept, size_t kept_bytes, void* workspace,
+                          float* logprobs, float* state, void* kept, size_t kept_bytes, void* workspace,
                           size_t workspace_bytes, void* stream) {
   int rc = check_common(N, D, V, dtype, index_dtype, inv_temperature);
   if (rc) return rc;
@@ -766,8 +769,8 @@ extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int i
   int* status = reinterpret_cast<int*>(ws + L.status);
   if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
   char* kp = static_cast<char*>(kept);
-  if (dtype == GH_BF16) return lsm_fwd_run<__nv_bfloat16>(H, W, N, D, V, dtype, sc2, L, kp, logprobs, lse2, ws, st);
-  return lsm_fwd_run<__half>(H, W, N, D, V, dtype, sc2, L, nullptr, logprobs, lse2, ws, st);
+  if (dtype == GH_BF16) return lsm_fwd_run<__nv_bfloat16>(H, W, N, D, V, dtype, sc2, L, kp, logprobs, state, ws, st);
+  return lsm_fwd_run<__half>(H, W, N, D, V, dtype, sc2, L, nullptr, logprobs, state, ws, st);
 }
 
 extern "C" int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V,
@@ -789,15 +792,15 @@ extern "C" int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, 
                           grad_weight, L, ws, st);
 }
 
-extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* logprobs,
-                          const float* lse2, const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
+extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* state,
+                          const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
                           int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
                           int fp32_grad_weight_accum, void* grad_input, void* grad_weight, void* workspace,
                           size_t workspace_bytes, void* stream) {
   int rc = check_common(N, D, V, dtype, index_dtype, inv_temperature);
   if (rc) return rc;
   if (N == 0) return GH_OK;
-  if (!H || !W || !index || !logprobs || !lse2 || !grad || !workspace)
+  if (!H || !W || !index || !state || !grad || !workspace)
     return set_error(GH_EINVAL, "null pointer argument");
   const BwdLayout L = bwd_layout(N, D, V, chunk_rows, false, fp32_grad_weight_accum);
   if (workspace_bytes < L.total)
@@ -806,6 +809,7 @@ extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int i
   char* ws = static_cast<char*>(workspace);
   const float inv_t = (float)inv_temperature;
   const float sc2 = (float)(inv_temperature * kLog2ed);
+  const float *lse2 = state, *logprobs = state + N;
   int* status = reinterpret_cast<int*>(ws + L.status);
   if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
   if (dtype == GH_BF16)

@@ -123,6 +123,11 @@ def clip_tensors(
             ws.numel(), _lib.stream_handle(device),
         )
         _lib.check(st, "clip_by_global_norm")
+        if outputs is not None:
+            try:  # what autograd saved of them is no longer what it was
+                torch.autograd.graph.increment_version(outputs)
+            except RuntimeError:  # inference tensors keep no count
+                pass
         for o, d in back:
             o.detach().copy_(d)
     return norm

@@ -82,10 +82,14 @@ def linear_logprobs(
     index: Tensor,
     ignore_index: int,
     temperature: float,
-    want_lse: bool = False,
+    want_state: bool = False,
     keep: bool = False,
 ) -> tuple[Tensor, Tensor | None, Tensor | None]:
-    """``(logprobs [N] fp32, lse2 [N] or None, kept (uint8) or None)``."""
+    """``(logprobs [N] fp32, state [2, N] or None, kept (uint8) or None)``.
+
+    One of the last two is what a backward needs: ``state`` (log-sum-exp in
+    log2 units, log-probabilities) for ``linear_logprobs_backward``, ``kept`` for
+    ``linear_logprobs_backward_kept``."""
     _validate(inputs, weight, index, temperature)
     N, D = inputs.shape
     V = weight.shape[0]
@@ -94,22 +98,22 @@ def linear_logprobs(
     with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax")
         out = torch.empty(N, dtype=torch.float32, device=dev)
-        lse2 = torch.empty(N, dtype=torch.float32, device=dev) if want_lse else None
+        state = torch.empty(2, N, dtype=torch.float32, device=dev) if want_state else None
         kept = torch.empty(kept_bytes(N, V), dtype=torch.uint8, device=dev) if keep else None
         if N == 0:
-            return out, lse2, kept
+            return out, state, kept
         x, w, idx = _operand(inputs), _operand(weight), index.contiguous()
         chunk = _chunk(N, D, V)
         ws = _lib.workspace(lib.gh_lsm_fwd_workspace_bytes(N, V, chunk, int(keep)), dev)
         st = lib.gh_lsm_fwd(
             x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), N, D, V,
             _lib.dtype_code(x.dtype), int(ignore_index), 1.0 / float(temperature), chunk, out.data_ptr(),
-            _lib.ptr(lse2), _lib.ptr(kept), 0 if kept is None else kept.numel(), ws.data_ptr(), ws.numel(),
+            _lib.ptr(state), _lib.ptr(kept), 0 if kept is None else kept.numel(), ws.data_ptr(), ws.numel(),
             _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax")
         _lib.raise_on_status(ws, "linear_selective_log_softmax")
-    return out, lse2, kept
+    return out, state, kept
 
 
 def _check_grad(grad: Tensor, inputs: Tensor) -> Tensor:
@@ -153,8 +157,7 @@ def linear_logprobs_backward(
     inputs: Tensor,
     weight: Tensor,
     index: Tensor,
-    logprobs: Tensor,
-    lse2: Tensor,
+    state: Tensor,
     grad: Tensor,
     ignore_index: int,
     temperature: float,
@@ -167,9 +170,8 @@ def linear_logprobs_backward(
     N, D = inputs.shape
     V = weight.shape[0]
     dev = inputs.device
-    for name, t in (("logprobs", logprobs), ("lse2", lse2)):
-        if t.shape != (N,) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"expected {name} as a contiguous fp32 tensor of shape {(N,)} on {dev}")
+    if state.shape != (2, N) or state.dtype != torch.float32 or state.device != dev or not state.is_contiguous():
+        raise ValueError(f"expected state as a contiguous fp32 tensor of shape {(2, N)} on {dev}")
     lib = _lib.load()
     with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax backward")
@@ -181,8 +183,8 @@ def linear_logprobs_backward(
         chunk = _chunk(N, D, V)
         ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, 0, int(fp32_grad_weight_accum)), dev)
         st = lib.gh_lsm_bwd(
-            x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), logprobs.data_ptr(),
-            lse2.data_ptr(), g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), int(ignore_index),
+            x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), state.data_ptr(),
+            g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), int(ignore_index),
             1.0 / float(temperature), chunk, int(fp32_grad_weight_accum), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(),
             ws.numel(), _lib.stream_handle(dev),
         )

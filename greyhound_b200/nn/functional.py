@@ -223,7 +223,8 @@ def chunked_linear_selective_log_softmax(
     out = cast(
         Tensor,
         ChunkedLinearSelectiveLogSoftmaxFunction.apply(
-            flat, weight, flat_index, ignore_index, float(temperature), grad_weight_accum_dtype == "fp32"
+            flat, weight, flat_index, ignore_index, float(temperature), grad_weight_accum_dtype == "fp32",
+            torch.is_grad_enabled(),
         ),
     )
     return out if inputs.ndim == 2 else out.reshape(index.shape)
@@ -271,7 +272,7 @@ def clipped_policy_loss(
     _no_grad_to(old_logprobs=old_logprobs, advantages=advantages, ref_logprobs=ref_logprobs)
     loss, state = ClippedPolicyLossFunction.apply(
         logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens,
-        (float(clip_low), float(clip_high), float(kl_multiplier), reduction, advantages_per),
+        (float(clip_low), float(clip_high), float(kl_multiplier), reduction, advantages_per), torch.is_grad_enabled(),
     )
     if not return_metrics:
         return cast(Tensor, loss)

@@ -70,6 +70,7 @@ def clip_grad_norm_(
     max_norm: float,
     norm_type: float = 2.0,
     error_if_nonfinite: bool = False,
+    foreach: bool | None = None,
 ) -> Tensor:
     """Clip the gradients of ``parameters`` in place to a global norm of ``max_norm``.
 
@@ -77,7 +78,8 @@ def clip_grad_norm_(
     without a gradient do not count. The gradients are scaled by
     ``min(1, max_norm / (norm + 1e-6))`` computed on the device: the call does
     not synchronise, except with ``error_if_nonfinite``, which reads the norm
-    and raises ``RuntimeError`` before any gradient has changed.
+    and raises ``RuntimeError`` before any gradient has changed. ``foreach`` is
+    accepted and makes no difference.
     Two parameters that share their gradient's memory raise ``ValueError``.
     """
     if isinstance(parameters, Tensor):

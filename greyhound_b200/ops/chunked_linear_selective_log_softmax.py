@@ -56,15 +56,15 @@ def linear_selective_log_softmax(
     ignore_index: int,
     temperature: float,
 ) -> tuple[Tensor, Tensor]:
-    """(logprobs [N], log-sum-exp in log2 units [N])."""
-    out, lse2, _ = linear_logprobs(inputs, weight, index, ignore_index, temperature, want_lse=True)
-    assert lse2 is not None
-    return out, lse2
+    """(logprobs [N], state [2, N]: log-sum-exp in log2 units, log-probabilities)."""
+    out, state, _ = linear_logprobs(inputs, weight, index, ignore_index, temperature, want_state=True)
+    assert state is not None
+    return out, state
 
 
 @linear_selective_log_softmax.register_fake
 def _(inputs, weight, index, ignore_index, temperature):
-    return _rows(inputs), _rows(inputs)
+    return _rows(inputs), torch.empty([2, inputs.shape[0]], dtype=torch.float32, device=inputs.device)
 
 
 @torch.library.custom_op("greyhound::linear_selective_log_softmax_kept", mutates_args=())
@@ -92,8 +92,7 @@ def linear_selective_log_softmax_bwd(
     inputs: Tensor,
     weight: Tensor,
     index: Tensor,
-    logprobs: Tensor,
-    lse2: Tensor,
+    state: Tensor,
     grad: Tensor,
     ignore_index: int,
     temperature: float,
@@ -103,15 +102,14 @@ def linear_selective_log_softmax_bwd(
 ) -> tuple[Tensor, Tensor]:
     """(grad_input [N, D], grad_weight [V, D]); an unwanted one is empty."""
     gi, gw = linear_logprobs_backward(
-        inputs, weight, index, logprobs, lse2, grad, ignore_index, temperature, fp32_grad_weight_accum,
-        want_input, want_weight,
+        inputs, weight, index, state, grad, ignore_index, temperature, fp32_grad_weight_accum, want_input,
+        want_weight,
     )
     return _present(gi, gw, inputs, weight)
 
 
 @linear_selective_log_softmax_bwd.register_fake
-def _(inputs, weight, index, logprobs, lse2, grad, ignore_index, temperature, fp32_grad_weight_accum, want_input,
-      want_weight):
+def _(inputs, weight, index, state, grad, ignore_index, temperature, fp32_grad_weight_accum, want_input, want_weight):
     return _grads(inputs, weight, want_input, want_weight)
 
 
@@ -145,9 +143,10 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
         ignore_index: int = -100,
         temperature: float = 1.0,
         fp32_grad_weight_accum: bool = True,
+        grad_enabled: bool = True,  # the caller's mode: in here gradients are always off
     ) -> Tensor:
         plain = _lib.eager(inputs) and _lib.eager(weight)
-        if not ctx.needs_input_grad[0] and not ctx.needs_input_grad[1]:
+        if not grad_enabled or not (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
             if plain:
                 return linear_logprobs(inputs, weight, index, ignore_index, temperature)[0]
             return linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)[0]
@@ -161,11 +160,11 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
             ctx.save_for_backward(inputs, weight, kept)
             return out
         if plain:
-            out, lse2, _ = linear_logprobs(inputs, weight, index, ignore_index, temperature, want_lse=True)
+            out, state, _ = linear_logprobs(inputs, weight, index, ignore_index, temperature, want_state=True)
         else:
-            out, lse2 = linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)
+            out, state = linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)
         ctx.ignore_index, ctx.fp32_accum = ignore_index, fp32_grad_weight_accum
-        ctx.save_for_backward(inputs, weight, index, out, lse2)
+        ctx.save_for_backward(inputs, weight, index, state)
         return out
 
     @staticmethod
@@ -179,10 +178,9 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
                 inputs, weight, kept, grad, ctx.temperature, want[0], want[1]
             )
         else:
-            inputs, weight, index, out, lse2 = ctx.saved_tensors
+            inputs, weight, index, state = ctx.saved_tensors
             bwd = linear_logprobs_backward if _lib.eager(grad) else linear_selective_log_softmax_bwd
             gi, gw = bwd(
-                inputs, weight, index, out, lse2, grad, ctx.ignore_index, ctx.temperature, ctx.fp32_accum,
-                want[0], want[1],
+                inputs, weight, index, state, grad, ctx.ignore_index, ctx.temperature, ctx.fp32_accum, want[0], want[1]
             )
-        return gi if want[0] else None, gw if want[1] else None, None, None, None, None
+        return gi if want[0] else None, gw if want[1] else None, None, None, None, None, None

@@ -92,8 +92,9 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         mask: Tensor | None,
         cu_seqlens: Tensor | None,
         options: tuple[float, float, float, str, str],  # the ops' arguments from clip_low to advantages_per
+        grad_enabled: bool = True,  # the caller's mode: in here gradients are always off
     ) -> tuple[Tensor, Tensor]:
-        want = ctx.needs_input_grad[0]
+        want = grad_enabled and ctx.needs_input_grad[0]
         fwd = policy_loss_forward if _lib.eager(logprobs) else clipped_policy_loss_fwd
         loss, state = fwd(logprobs, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, *options, want)
         if want:
@@ -107,10 +108,10 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_output: Tensor, _: Tensor):  # type: ignore[override]
         if grad_output is None:
-            return (None,) * 7
+            return (None,) * 8
         state, cu = ctx.saved_tensors
         bwd = policy_loss_backward if _lib.eager(state) else clipped_policy_loss_bwd
-        return bwd(state, cu, grad_output, *ctx.like), None, None, None, None, None, None
+        return bwd(state, cu, grad_output, *ctx.like), None, None, None, None, None, None, None
 
 
 @torch.library.custom_op("greyhound::preference_loss_fwd", mutates_args=())

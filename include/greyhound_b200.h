@@ -338,7 +338,8 @@ GH_API int gh_scale(const void* in, void* out, int64_t n, int dtype, const float
  *   index [N] in {I32, I64}: rows equal to ignore_index give 0 and no
  *           gradient; an index outside [0, V) gives NaN, no gradient, and
  *           GH_DEV_BAD_LABEL
- *   lse2    [N] log-sum-exp in log2 units (optional; gh_lsm_bwd needs it)
+ *   state   [2, N] log-sum-exp in log2 units, and the log-probabilities once
+ *           more (optional; gh_lsm_bwd needs it)
  *   kept    optional (BF16), gh_lsm_kept_bytes(): e^x in 16 bits and the row
  *           factors, which gh_lsm_bwd_kept reads (any number of times)
  * The backward takes the gradient `grad` [N] (F32) of logprobs and writes
@@ -353,14 +354,14 @@ GH_API size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_
                                          int fp32_grad_weight_accum);
 GH_API int gh_lsm_fwd(const void* H, const void* W, const void* index, int index_dtype, int64_t N, int64_t D,
                       int64_t V, int dtype, int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
-                      float* logprobs, float* lse2, void* kept, size_t kept_bytes, void* workspace,
+                      float* logprobs, float* state, void* kept, size_t kept_bytes, void* workspace,
                       size_t workspace_bytes, void* stream);
 GH_API int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V,
                            int dtype, double inv_temperature, const void* kept, size_t kept_bytes,
                            void* grad_input, void* grad_weight, void* workspace, size_t workspace_bytes,
                            void* stream);
-GH_API int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* logprobs,
-                      const float* lse2, const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
+GH_API int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* state,
+                      const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
                       int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
                       int fp32_grad_weight_accum, void* grad_input, void* grad_weight, void* workspace,
                       size_t workspace_bytes, void* stream);

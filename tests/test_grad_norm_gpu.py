@@ -227,3 +227,27 @@ def test_deterministic_and_capturable():
     torch.cuda.synchronize()
     for outs, norm in results:
         assert torch.equal(norm, n) and all(torch.equal(a, b) for a, b in zip(want, outs))
+
+
+@requires_gpu
+def test_more_than_2_to_the_31_elements():
+    n = (1 << 31) + 24
+    t = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    t[-1], t[1 << 31] = 3.0, 5.0
+    want = math.sqrt(n + 8 + 24)
+    outs, norm = clip_by_global_norm([t], want / 2, out=[t])
+    assert abs(norm.item() - want) <= E * want
+    assert outs[0][0] == 0.5 and outs[0][-1] == 1.5 and outs[0][1 << 31] == 2.5
+    assert t[(1 << 31) + 1 : -1].eq(0.5).all() and t[: 1 << 20].eq(0.5).all()
+
+
+@requires_gpu
+def test_autograd_notices_clipping_in_place():
+    x = torch.randn(1000, device="cuda", requires_grad=True)
+    y = x.detach().clone()
+    z = (x * y).sum()
+    clip_by_global_norm([y], 0.1, out=[y])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():
+        clip_by_global_norm([y.clone()], 0.1, out=[torch.empty_like(y)])

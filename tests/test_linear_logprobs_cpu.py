@@ -54,7 +54,7 @@ def test_c_entries_refuse_bad_arguments():
         (fwd(dtype=_lib.GH_F16, kept=8, kb=1 << 20), RuntimeError),
         (lib.gh_lsm_bwd_kept(8, 8, 8, 4, 16, 9, _lib.GH_F16, 1.0, 8, 1 << 20, 8, 8, 8, 1 << 30, None), RuntimeError),
         (lib.gh_lsm_bwd_kept(8, 8, 8, 4, 16, 9, _lib.GH_BF16, 1.0, 8, 1 << 20, 8, 8, 8, 16, None), RuntimeError),
-        (lib.gh_lsm_bwd(8, 8, None, _lib.GH_I64, 8, 8, 8, 4, 16, 9, _lib.GH_BF16, -100, 1.0, 4, 1, 8, 8, 8, 1 << 30, None), ValueError),
+        (lib.gh_lsm_bwd(8, 8, None, _lib.GH_I64, 8, 8, 4, 16, 9, _lib.GH_BF16, -100, 1.0, 4, 1, 8, 8, 8, 1 << 30, None), ValueError),
     ):
         with pytest.raises(error):
             _lib.check(st, "x")

@@ -310,8 +310,8 @@ def test_opcheck():
     H, W, t, g = make(40, 64, 130, torch.bfloat16, 16)
     opcheck(linear_selective_log_softmax, (H, W, t, -100, 1.0))
     opcheck(linear_selective_log_softmax_kept, (H, W, t, -100, 1.0), test_utils=["test_schema", "test_faketensor"])
-    y, lse2 = linear_selective_log_softmax(H, W, t, -100, 1.0)
-    opcheck(linear_selective_log_softmax_bwd, (H, W, t, y, lse2, g, -100, 1.0, True, True, False))
+    _, state = linear_selective_log_softmax(H, W, t, -100, 1.0)
+    opcheck(linear_selective_log_softmax_bwd, (H, W, t, state, g, -100, 1.0, True, True, False))
     _, kept = linear_selective_log_softmax_kept(H, W, t, -100, 1.0)
     opcheck(linear_selective_log_softmax_kept_bwd, (H, W, kept, g, 1.0, True, True))
 
@@ -379,3 +379,32 @@ def test_large_products(N, V):
         rW = d.T @ H.double()
         bW = (3 * u * d.abs() + ey * gg.abs() * p).T @ H.double().abs() + 2 * u * rW.abs()
         assert ((dw[cols].double() - rW).abs() <= bW + 2.0**-62 * (gg.abs() * H.double().abs()).sum(0)).all()
+
+
+@requires_gpu
+def test_scoring_with_trainable_weights_stores_nothing():
+    """torch.no_grad with parameters that require a gradient: no e^x is kept (here it would be 200 MB)."""
+    H, W, t, _ = make(1000, 64, 100_000, torch.bfloat16, 22)
+    w = torch.nn.Parameter(W)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            chunked_linear_selective_log_softmax(H, w, t)
+            torch.cuda.synchronize()
+            base = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            y = chunked_linear_selective_log_softmax(H, w, t)
+            assert torch.cuda.max_memory_allocated() - base < 16 << 20
+    assert torch.equal(y, chunked_linear_selective_log_softmax(H, w, t).detach())
+
+
+@requires_gpu
+@pytest.mark.parametrize("kept", [True, False])
+def test_result_may_be_changed_in_place(monkeypatch, kept):
+    if not kept:
+        monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    H, W, t, g = make(50, 64, 300, torch.bfloat16, 23)
+    _, dh, _ = check(H, W, t, g)
+    h = H.clone().requires_grad_(True)
+    y = chunked_linear_selective_log_softmax(h, W, t)
+    y.mul_(2.0)
+    assert torch.allclose(torch.autograd.grad(y, h, g / 2)[0].float(), dh.float(), rtol=2.0**-7, atol=1e-6)

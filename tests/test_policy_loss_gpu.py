@@ -302,3 +302,13 @@ def test_captured_and_on_another_stream(lengths):
         out.zero_()
         graph.replay()
         assert torch.equal(out, grad)
+
+
+@requires_gpu
+def test_without_gradients():
+    b = batch([300, 5], torch.float32, 13, False)
+    loss, _ = check(b, "mean")
+    lp = b["lp"].clone().requires_grad_(True)
+    with torch.no_grad():
+        got = clipped_policy_loss(lp, b["old"], b["adv"], mask=b["mask"], cu_seqlens=b["cu"], clip_high=0.3)
+    assert torch.equal(got, loss) and not got.requires_grad
