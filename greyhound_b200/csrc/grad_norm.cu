@@ -22,6 +22,7 @@
 // norm, too.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "common.cuh"
@@ -44,7 +45,9 @@ struct List {
   int count;
 };
 constexpr int kMaxTensors = 896;  // 32 KB of kernel arguments at most
-constexpr int kFewTensors = 96;   // a list that costs less to hand over
+// shorter lists cost less to hand over
+constexpr int kSomeTensors = 288;
+constexpr int kFewTensors = 96;
 static_assert(sizeof(List<kMaxTensors>) + 128 <= 32764, "kernel arguments");
 
 // Tensor of a chunk: the last one that starts at or before it.
@@ -344,14 +347,15 @@ int scale_lists(const Call& c, const double* part, int parts, double max_norm, i
 
 template <typename A>
 int run_call(const Call& c, double max_norm, int in_place, float* norm, double* part, int max_parts, cudaStream_t st) {
-  int parts = 0;
-  int rc;
-  if (c.count <= kFewTensors) {
-    if ((rc = norm_lists<A, kFewTensors>(c, part, &parts, max_parts, st))) return rc;
-    return scale_lists<A, kFewTensors>(c, part, parts, max_norm, in_place, norm, st);
-  }
-  if ((rc = norm_lists<A, kMaxTensors>(c, part, &parts, max_parts, st))) return rc;
-  return scale_lists<A, kMaxTensors>(c, part, parts, max_norm, in_place, norm, st);
+  auto both = [&](auto max) {
+    constexpr int MAX = decltype(max)::value;
+    int parts = 0;
+    const int rc = norm_lists<A, MAX>(c, part, &parts, max_parts, st);
+    return rc ? rc : scale_lists<A, MAX>(c, part, parts, max_norm, in_place, norm, st);
+  };
+  if (c.count <= kFewTensors) return both(std::integral_constant<int, kFewTensors>{});
+  if (c.count <= kSomeTensors) return both(std::integral_constant<int, kSomeTensors>{});
+  return both(std::integral_constant<int, kMaxTensors>{});
 }
 
 struct Span {

@@ -65,9 +65,9 @@ def test_norm_and_clip(shapes, dtypes, kind):
 
 
 @requires_gpu
-@pytest.mark.parametrize("count", [96, 97, 895, 896, 897, 2000])
+@pytest.mark.parametrize("count", [96, 97, 288, 289, 896, 897, 2000])
 def test_long_lists(count):
-    """One launch holds 96 or 896 tensors."""
+    """One launch holds 96, 288 or 896 tensors."""
     ts = make([(i % 40 + 1,) for i in range(count)], TYPES, count)
     check_clip(ts, 0.5 * norm64(ts))
     ref = [t.clone() for t in ts]
