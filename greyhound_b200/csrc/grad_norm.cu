@@ -430,6 +430,7 @@ extern "C" int gh_clip_by_global_norm(const void* const* tensors, void* const* o
     }
   }
   if (workspace_bytes < gh_global_norm_workspace_bytes(count)) return set_error(GH_EWORKSPACE, "workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return set_error(GH_EINVAL, "workspace must be 8-byte aligned");
   double* part = static_cast<double*>(workspace);
   const int max_parts = (int)((workspace_bytes - 256) / sizeof(double));
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -21,6 +21,8 @@
 //              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, 2 GB of
 //              workspace whatever N, and fp16 (whose exponent cannot hold e^x).
 // Bound by the tensor pipe for many rows and by reading W once for few.
+#include <initializer_list>
+
 #include "row_ops.cuh"
 #include "tc_gemm_host.cuh"
 
@@ -578,6 +580,14 @@ int check_common(int64_t N, int64_t D, int64_t V, int dtype, int index_dtype, do
   return GH_OK;
 }
 
+// What vector loads, bulk copies and 8-byte stores take for granted.
+int check_aligned(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & 15)
+      return set_error(GH_EINVAL, "operands, gradients and buffers need 16-byte aligned addresses");
+  return GH_OK;
+}
+
 template <typename T>
 int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, int dtype, float sc2,
                 const FwdLayout& L, char* kept, float* y, float* state, char* ws, cudaStream_t st) {
@@ -758,6 +768,7 @@ extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int i
   if (rc) return rc;
   if (N == 0) return GH_OK;
   if (!H || !W || !index || !logprobs || !workspace) return set_error(GH_EINVAL, "null pointer argument");
+  if ((rc = check_aligned({H, W, kept, workspace}))) return rc;
   if (kept && dtype != GH_BF16) return set_error(GH_EUNSUPPORTED, "only bf16 operands keep e^x");
   if (kept && kept_bytes < kept_layout(N, V).total) return set_error(GH_EWORKSPACE, "kept buffer too small");
   const FwdLayout L = fwd_layout(N, V, chunk_rows, kept != nullptr);
@@ -782,6 +793,7 @@ extern "C" int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, 
   if (dtype != GH_BF16) return set_error(GH_EUNSUPPORTED, "only bf16 operands keep e^x");
   if (N == 0) return GH_OK;
   if (!H || !W || !grad || !kept || !workspace) return set_error(GH_EINVAL, "null pointer argument");
+  if ((rc = check_aligned({H, W, kept, grad_input, grad_weight, workspace}))) return rc;
   if (kept_bytes < kept_layout(N, V).total) return set_error(GH_EWORKSPACE, "kept buffer too small");
   const BwdLayout L = bwd_layout(N, D, V, N, true, true);
   if (workspace_bytes < L.total)
@@ -802,6 +814,7 @@ extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int i
   if (N == 0) return GH_OK;
   if (!H || !W || !index || !state || !grad || !workspace)
     return set_error(GH_EINVAL, "null pointer argument");
+  if ((rc = check_aligned({H, W, grad_input, grad_weight, workspace}))) return rc;
   const BwdLayout L = bwd_layout(N, D, V, chunk_rows, false, fp32_grad_weight_accum);
   if (workspace_bytes < L.total)
     return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);

@@ -750,6 +750,7 @@ extern "C" int gh_policy_loss_fwd(const void* logprobs, int dtype, const void* o
   const PolicyLayout L = policy_layout(tokens, seqs, reduction);
   if (workspace_bytes < L.total)
     return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return set_error(GH_EINVAL, "workspace must be 8-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Policy p;
   p.lp = logprobs;
@@ -791,6 +792,7 @@ extern "C" int gh_policy_loss_bwd(const float* dlogprobs, const float* scal, con
   if (!dlogprobs || !scal || !grad_output || !grad || !workspace) return set_error(GH_EINVAL, "null pointer argument");
   const PolicyLayout L = policy_layout(tokens, seqs, reduction);
   if (workspace_bytes < L.total) return set_error(GH_EWORKSPACE, "workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return set_error(GH_EINVAL, "workspace must be 8-byte aligned");
   const Sums* per_seq =
       reduction == RED_SEQ_MEAN ? reinterpret_cast<const Sums*>(static_cast<const char*>(workspace) + L.seqs) : nullptr;
   const Cut c = cut_tokens(tokens, seqs, false);
@@ -825,6 +827,7 @@ extern "C" int gh_preference_loss_fwd(const void* logprobs, int dtype, const voi
   const PrefLayout L = pref_layout(tokens, seqs);
   if (workspace_bytes < L.total)
     return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return set_error(GH_EINVAL, "workspace must be 8-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Pref p;
   p.lp = logprobs;

@@ -334,7 +334,8 @@ GH_API int gh_scale(const void* in, void* out, int64_t n, int dtype, const float
  * log-probabilities start from logits, kernels/logprobs.py:131):
  *   x = H W^T * inv_temperature; logprobs[r] = x[r, index[r]] - logsumexp(x[r])
  * in fp32 from the fp32 accumulator, without the [N, V] logits in memory.
- *   H [N, D], W [V, D] in {F16, BF16}, D % 8 == 0, 16-byte aligned
+ *   H [N, D], W [V, D] in {F16, BF16}, D % 8 == 0; they, kept, the gradients
+ *           and the workspace 16-byte aligned
  *   index [N] in {I32, I64}: rows equal to ignore_index give 0 and no
  *           gradient; an index outside [0, V) gives NaN, no gradient, and
  *           GH_DEV_BAD_LABEL
@@ -374,7 +375,7 @@ GH_API int gh_lsm_bwd(const void* H, const void* W, const void* index, int index
  * [0, tokens] set GH_DEV_BAD_SEQLENS in the device's sticky slot; the results
  * are then unspecified. mask [tokens] (bytes, optional): 0 leaves a token out,
  * whatever its values; a token outside every sequence is left out, too, and
- * the gradient of one left out is 0.
+ * the gradient of one left out is 0. The workspace is 8-byte aligned.
  * logprobs [tokens] in {F16, BF16, F32}; the other log-probabilities in the same
  * type or F32 (other_dtype). Results are F32 scalars unless stated.
  *

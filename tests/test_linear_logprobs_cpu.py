@@ -42,19 +42,39 @@ def test_refusals(args, kw, error, match):
 
 def test_c_entries_refuse_bad_arguments():
     lib = _lib.load()
-    fwd = lambda dtype=_lib.GH_BF16, D=16, kept=None, kb=0, wb=1 << 30, inv_t=1.0, idt=_lib.GH_I64: lib.gh_lsm_fwd(  # noqa: E731
-        8, 8, 8, idt, 4, D, 9, dtype, -100, inv_t, 4, 8, 8, kept, kb, 8, wb, None)
+    BFC, F16, I64 = _lib.GH_BF16, _lib.GH_F16, _lib.GH_I64
+
+    def fwd(dtype=BFC, D=16, kept=None, kb=0, wb=1 << 30, inv_t=1.0, idt=I64, H=16, W=16, ws=16):
+        return lib.gh_lsm_fwd(H, W, 8, idt, 4, D, 9, dtype, -100, inv_t, 4, 8, None, kept, kb, ws, wb, None)
+
+    def kept_bwd(dtype=BFC, wb=1 << 30, H=16, gi=16, gw=16, kept=16, kb=1 << 20):
+        return lib.gh_lsm_bwd_kept(H, 16, 8, 4, 16, 9, dtype, 1.0, kept, kb, gi, gw, 16, wb, None)
+
+    def bwd(index=8, wb=1 << 30, W=16, gi=16):
+        return lib.gh_lsm_bwd(16, W, index, I64, 8, 8, 4, 16, 9, BFC, -100, 1.0, 4, 1, gi, 16, 16, wb, None)
+
     for st, error in (
         (fwd(dtype=_lib.GH_F32), TypeError),
         (fwd(idt=_lib.GH_F32), TypeError),
         (fwd(D=12), ValueError),
         (fwd(inv_t=0.0), ValueError),
         (fwd(wb=16), RuntimeError),
-        (fwd(kept=8, kb=16), RuntimeError),
-        (fwd(dtype=_lib.GH_F16, kept=8, kb=1 << 20), RuntimeError),
-        (lib.gh_lsm_bwd_kept(8, 8, 8, 4, 16, 9, _lib.GH_F16, 1.0, 8, 1 << 20, 8, 8, 8, 1 << 30, None), RuntimeError),
-        (lib.gh_lsm_bwd_kept(8, 8, 8, 4, 16, 9, _lib.GH_BF16, 1.0, 8, 1 << 20, 8, 8, 8, 16, None), RuntimeError),
-        (lib.gh_lsm_bwd(8, 8, None, _lib.GH_I64, 8, 8, 4, 16, 9, _lib.GH_BF16, -100, 1.0, 4, 1, 8, 8, 8, 1 << 30, None), ValueError),
+        (fwd(kept=16, kb=16), RuntimeError),
+        (fwd(dtype=F16, kept=16, kb=1 << 20), RuntimeError),
+        (fwd(H=8), ValueError),
+        (fwd(W=2), ValueError),
+        (fwd(ws=8), ValueError),
+        (fwd(H=None), ValueError),
+        (kept_bwd(dtype=F16), RuntimeError),
+        (kept_bwd(wb=16), RuntimeError),
+        (kept_bwd(kb=16), RuntimeError),
+        (kept_bwd(H=8), ValueError),
+        (kept_bwd(gi=8), ValueError),
+        (kept_bwd(gw=2), ValueError),
+        (bwd(index=None), ValueError),
+        (bwd(wb=16), RuntimeError),
+        (bwd(W=4), ValueError),
+        (bwd(gi=4), ValueError),
     ):
         with pytest.raises(error):
             _lib.check(st, "x")
