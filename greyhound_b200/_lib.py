@@ -95,15 +95,15 @@ SIGNATURES: dict[str, tuple] = {
     "gh_memcpy_async": (_i32, [_vp, _vp, _sz, _vp]),
     "gh_take_device_errors": (_i32, [_i32]),
     "gh_ce_noalloc_status": (_i32, [ctypes.POINTER(ctypes.c_int), _vp]),
-    "gh_lsm_kept_bytes": (_sz, [_i64, _i64]),
+    "gh_lsm_kept_bytes": (_sz, [_i64, _i64, _i32]),
     "gh_lsm_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
-    "gh_lsm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, _i32]),
+    "gh_lsm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, _i32, _i32]),
     "gh_lsm_fwd": (
         _i32,
         [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _i64, _f64, _i64, _vp, _vp, _vp, _sz, _vp, _sz, _vp],
     ),
     "gh_lsm_bwd_kept": (
-        _i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _f64, _vp, _sz, _vp, _vp, _vp, _sz, _vp]
+        _i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _f64, _i64, _i32, _vp, _sz, _vp, _vp, _vp, _sz, _vp]
     ),
     "gh_lsm_bwd": (
         _i32,

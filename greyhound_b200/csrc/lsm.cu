@@ -13,13 +13,16 @@
 // nothing per row.
 //
 // Two backward forms:
-//   kept       (bf16) the forward's epilogue also stores q = e^x in 16 bits. With
+//   kept       the forward's epilogue also stores q = e^x in 16 bits. In bf16, with
 //              a[r] = -g[r] / temperature * e^-lse[r], d = a (q - e^lse onehot):
 //              the one-hot part goes into q's target column, a into dH's epilogue
 //              and into a 16-bit copy of H for dW. Three GEMMs for both passes.
+//              fp16's exponent cannot hold e^x: every 128-column group of a row is
+//              stored relative to its largest value, and a pass over a chunk of
+//              rows turns that into d.
 //   recomputed the backward repeats the logits GEMM row chunk by row chunk with an
-//              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, 2 GB of
-//              workspace whatever N, and fp16 (whose exponent cannot hold e^x).
+//              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, but 2 GB of
+//              workspace whatever N.
 // Bound by the tensor pipe for many rows and by reading W once for few.
 #include <initializer_list>
 
@@ -296,7 +299,7 @@ lsm_rows_kernel(const __nv_bfloat16* __restrict__ H, const float* __restrict__ g
   }
 }
 
-// Backward, recomputed form, fp16: d is written times 2^k so that the largest
+// Backward, fp16: d is written times 2^k so that the largest
 // row factor lies in [2^13, 2^14): (onehot - p) keeps 2^-38 of the largest
 // gradient instead of fp16's 2^-24. scale = {2^k, 2^-k}; non-finite gradients
 // do not count.
@@ -322,7 +325,7 @@ lsm_gscale_kernel(const float* __restrict__ g, const int* __restrict__ tgt, int6
   }
 }
 
-// Row factor and target value of EPI_LSM_GRAD for all rows.
+// Row factor and target value of d for all rows.
 __global__ void __launch_bounds__(256)
 lsm_factor_kernel(const float* __restrict__ g, const float* __restrict__ y, const int* __restrict__ tgt, float inv_t,
                   const float* __restrict__ scale, int64_t rows, float* __restrict__ rfac, float* __restrict__ tval) {
@@ -333,8 +336,44 @@ lsm_factor_kernel(const float* __restrict__ g, const float* __restrict__ y, cons
   tval[r] = tgt[r] >= 0 ? -f * expm1f(y[r]) : 0.f;
 }
 
+// Backward, kept form in fp16: d = rfac (onehot - q 2^(shift - lse2)), 8 columns
+// at a time (of one group, whose 128 columns share a shift); grid (rows, column
+// chunks). Reads and writes the chunk once: 15 us for 777 x 32003, where the GEMM
+// that recomputes it takes 70.
+__global__ void __launch_bounds__(256)
+lsm_unpack_kernel(const __half* __restrict__ q, int64_t ldq, const float* __restrict__ gmax, int64_t N,
+                  const float* __restrict__ lse2, const float* __restrict__ rfac, const float* __restrict__ tval,
+                  const int* __restrict__ tgt, int64_t V, __half* __restrict__ d) {
+  const int64_t r = blockIdx.x;
+  const int t = tgt[r];
+  const float f = rfac[r], l2 = lse2[r], tv = tval[r];
+  const int64_t vecs = ldq / 8;  // the pitch: columns past V hold nothing and are read by nobody
+  const __half* qr = q + r * ldq;
+  __half* dr = d + r * ldq;
+  for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < vecs; i += (int64_t)gridDim.y * 256) {
+    Vec16<__half> v;
+    if (t < 0) {
+      v.raw = make_uint4(0, 0, 0, 0);  // a row left out: 0 even where q is NaN
+    } else {
+      v.raw = ld16_last(reinterpret_cast<const uint4*>(qr) + i);
+      const float w = -f * fast_exp2(gmax[(i >> 4) * N + r] - l2);
+      float x[8];
+      v.to_float(x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= w;
+      if (t >> 3 == (int)i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if ((t & 7) == k) x[k] = tv;
+      }
+      v.from_float(x);
+    }
+    st16(reinterpret_cast<uint4*>(dr) + i, v.raw);
+  }
+}
+
 // H with left-out rows zeroed (0 * NaN must not reach dW): the dW GEMM's second
-// operand in the recomputed form.
+// operand where d is written out.
 __global__ void __launch_bounds__(256)
 lsm_clean_rows_kernel(const uint4* __restrict__ H, const int* __restrict__ tgt, int64_t rows, int64_t vpr,
                       uint4* __restrict__ out) {
@@ -466,17 +505,24 @@ FwdLayout fwd_layout(int64_t N, int64_t V, int64_t chunk, bool keep) {
   return L;
 }
 
-// What the kept form holds between the passes: q and the row factors.
+// What the kept form holds between the passes: q and, in bf16, the row factors;
+// in fp16 the groups' shifts and the rows' log-sum-exp, log-probability, target.
 struct KeptLayout {
-  size_t q = 0, alpha0, total;
+  size_t q = 0, alpha0 = 0, gmax = 0, lse2 = 0, y = 0, tgt = 0, total;
   int64_t ldq;
 };
-KeptLayout kept_layout(int64_t N, int64_t V) {
+KeptLayout kept_layout(int64_t N, int64_t V, int dtype) {
   KeptLayout L;
   L.ldq = (V + 7) / 8 * 8;  // 16-byte row pitch for TMA
   size_t off = al256((size_t)N * L.ldq * 2);
-  L.alpha0 = off;
-  off = al256(off + sizeof(float) * N);
+  if (dtype == GH_BF16) {
+    L.alpha0 = off; off = al256(off + sizeof(float) * N);
+  } else {
+    L.gmax = off;   off = al256(off + sizeof(float) * N * 2 * (size_t)((V + BN - 1) / BN));
+    L.lse2 = off;   off = al256(off + sizeof(float) * N);
+    L.y = off;      off = al256(off + sizeof(float) * N);
+    L.tgt = off;    off = al256(off + sizeof(int) * N);
+  }
   L.total = off;
   return L;
 }
@@ -486,6 +532,7 @@ struct BwdLayout {
   int64_t chunk, ldd;
   bool need_acc;
 };
+// kept: the bf16 form that needs no d.
 BwdLayout bwd_layout(int64_t N, int64_t D, int64_t V, int64_t chunk, bool kept, bool fp32_accum) {
   BwdLayout L;
   if (kept || chunk <= 0 || chunk > N) chunk = N;
@@ -591,12 +638,15 @@ int check_aligned(std::initializer_list<const void*> ptrs) {
 template <typename T>
 int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, int dtype, float sc2,
                 const FwdLayout& L, char* kept, float* y, float* state, char* ws, cudaStream_t st) {
+  constexpr bool kHalf = gemm::AbType<T>::v == 0;
   int* status = reinterpret_cast<int*>(ws + L.status);
-  int* tgt = reinterpret_cast<int*>(ws + L.tgt);
-  float* lse2 = state ? state : reinterpret_cast<float*>(ws + L.lse2);
+  const KeptLayout K = kept_layout(N, V, dtype);
+  const bool own_state = kHalf && kept;
+  const int* tgt = reinterpret_cast<const int*>(own_state ? kept + K.tgt : ws + L.tgt);
+  float* lse2 = own_state ? reinterpret_cast<float*>(kept + K.lse2) : state ? state : reinterpret_cast<float*>(ws + L.lse2);
+  float* y2 = own_state ? reinterpret_cast<float*>(kept + K.y) : state ? state + N : nullptr;
   float* xt = reinterpret_cast<float*>(ws + L.xt);
   float2* stats = reinterpret_cast<float2*>(ws + L.stats);
-  const KeptLayout K = kept_layout(N, V);
   int* slot = nullptr;
   int rc = device_error_slot(&slot);
   if (rc) return rc;
@@ -611,24 +661,24 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
     CombineOut o{};
     o.y = y + s0;
     o.lse2 = lse2 + s0;
-    o.y2 = state ? state + N + s0 : nullptr;
+    o.y2 = y2 ? y2 + s0 : nullptr;
     o.status = status;
     o.slot = s0 + rows >= N ? slot : nullptr;
     const void* Hc = static_cast<const T*>(H) + s0 * D;
-    if constexpr (sizeof(T) == 2 && gemm::AbType<T>::v == 1) {
-      if (kept) {
-        p.out = kept + K.q;
-        p.ldo = K.ldq;
-        p.vec_ok = 1;
+    if (kept) {
+      p.out = kept + K.q;
+      p.ldo = K.ldq;
+      p.vec_ok = 1;
+      p.gmax = reinterpret_cast<float*>(kHalf ? kept + K.gmax : ws + L.gmax);
+      if (!kHalf) {
         p.qmode = reinterpret_cast<uint8_t*>(ws + L.qmode);
-        p.gmax = reinterpret_cast<float*>(ws + L.gmax);
         o.q = reinterpret_cast<__nv_bfloat16*>(kept + K.q);
         o.ldq = K.ldq;
         o.qmode = p.qmode;
         o.gmax = p.gmax;
         o.alpha0 = reinterpret_cast<float*>(kept + K.alpha0);
-        if ((rc = logits_gemm<T, gemm::EPI_LSM_Q>(Hc, W, rows, D, V, dtype, p, st))) return rc;
       }
+      if ((rc = logits_gemm<T, gemm::EPI_LSM_Q>(Hc, W, rows, D, V, dtype, p, st))) return rc;
     }
     int parts = L.num_n;
     if (!kept) {
@@ -654,7 +704,7 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
 int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V, float inv_t,
                      const char* kept, void* dH, void* dW, const BwdLayout& L, char* ws, cudaStream_t st) {
   int* status = reinterpret_cast<int*>(ws + L.status);
-  const KeptLayout K = kept_layout(N, V);
+  const KeptLayout K = kept_layout(N, V, GH_BF16);
   const int sms = num_sms_dev();
   int* slot = nullptr;
   int rc = device_error_slot(&slot);
@@ -676,12 +726,13 @@ int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N,
   return dH && dh_slices(N, D, V) ? GH_OK : publish_status(status, st);
 }
 
+// d chunk by chunk, recomputed or (kept, fp16) from the stored q, and its products.
 template <typename T>
-int lsm_bwd_run(const void* H, const void* W, const float* y, const float* lse2, const float* grad, int64_t N,
-                int64_t D, int64_t V, int dtype, float inv_t, float sc2, void* dH, void* dW, bool fp32_accum,
-                const BwdLayout& L, char* ws, cudaStream_t st) {
+int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, const float* lse2, const float* grad,
+                int64_t N, int64_t D, int64_t V, int dtype, float inv_t, float sc2, const char* kept, void* dH, void* dW,
+                bool fp32_accum, const BwdLayout& L, char* ws, cudaStream_t st) {
   int* status = reinterpret_cast<int*>(ws + L.status);
-  int* tgt = reinterpret_cast<int*>(ws + L.tgt);
+  const KeptLayout K = kept_layout(N, V, dtype);
   float* rfac = reinterpret_cast<float*>(ws + L.rfac);
   float* tval = reinterpret_cast<float*>(ws + L.tval);
   float* acc = reinterpret_cast<float*>(ws + L.acc);
@@ -704,17 +755,30 @@ int lsm_bwd_run(const void* H, const void* W, const float* y, const float* lse2,
     const int64_t rows = s0 + L.chunk <= N ? L.chunk : N - s0;
     const bool first = s0 == 0, last = s0 + rows >= N;
     const T* Hc = static_cast<const T*>(H) + s0 * D;
-    gemm::Params p{};
-    p.tgt = tgt + s0;
-    p.sc2 = sc2;
-    p.lse2 = lse2 + s0;
-    p.rfac = rfac + s0;
-    p.tval = tval + s0;
-    p.out = d;
-    p.ldo = L.ldd;
-    p.vec_ok = 1;
-    p.status = status;
-    if ((rc = logits_gemm<T, gemm::EPI_LSM_GRAD>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+    if (kept) {
+      // columns shared out so that few rows fill the SMs, too
+      int64_t cols = (8 * (int64_t)sms + rows - 1) / rows, most = (L.ldd / 8 + 255) / 256;
+      if (cols > most) cols = most;
+      if (cols > 65535) cols = 65535;
+      lsm_unpack_kernel<<<dim3((unsigned)rows, (unsigned)cols), 256, 0, st>>>(
+          reinterpret_cast<const __half*>(kept + K.q) + s0 * K.ldq, K.ldq,
+          reinterpret_cast<const float*>(kept + K.gmax) + s0, N, lse2 + s0, rfac + s0, tval + s0, tgt + s0, V,
+          reinterpret_cast<__half*>(d));
+      count_launch(1);
+      if ((rc = check_launch("lsm_unpack"))) return rc;
+    } else {
+      gemm::Params p{};
+      p.tgt = tgt + s0;
+      p.sc2 = sc2;
+      p.lse2 = lse2 + s0;
+      p.rfac = rfac + s0;
+      p.tval = tval + s0;
+      p.out = d;
+      p.ldo = L.ldd;
+      p.vec_ok = 1;
+      p.status = status;
+      if ((rc = logits_gemm<T, gemm::EPI_LSM_GRAD>(Hc, W, rows, D, V, dtype, p, st))) return rc;
+    }
     if (dW) {
       lsm_clean_rows_kernel<<<4 * sms, 256, 0, st>>>(reinterpret_cast<const uint4*>(Hc), tgt + s0, rows, D / 8,
                                                      reinterpret_cast<uint4*>(hs));
@@ -747,17 +811,19 @@ int lsm_bwd_run(const void* H, const void* W, const float* y, const float* lse2,
 
 using namespace gh;
 
-extern "C" size_t gh_lsm_kept_bytes(int64_t N, int64_t V) {
-  return N < 0 || V <= 0 ? 0 : kept_layout(N, V).total;
+extern "C" size_t gh_lsm_kept_bytes(int64_t N, int64_t V, int dtype) {
+  return N < 0 || V <= 0 || elt_size(dtype) != 2 ? 0 : kept_layout(N, V, dtype).total;
 }
 
 extern "C" size_t gh_lsm_fwd_workspace_bytes(int64_t N, int64_t V, int64_t chunk_rows, int keep) {
   return N < 0 || V <= 0 ? 0 : fwd_layout(N, V, chunk_rows, keep != 0).total;
 }
 
-extern "C" size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t chunk_rows, int kept,
+// A kept bf16 backward needs neither chunks nor d.
+extern "C" size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t chunk_rows, int dtype, int kept,
                                              int fp32_grad_weight_accum) {
-  return N < 0 || D <= 0 || V <= 0 ? 0 : bwd_layout(N, D, V, chunk_rows, kept != 0, fp32_grad_weight_accum).total;
+  if (N < 0 || D <= 0 || V <= 0) return 0;
+  return bwd_layout(N, D, V, chunk_rows, kept && dtype == GH_BF16, fp32_grad_weight_accum).total;
 }
 
 extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int index_dtype, int64_t N, int64_t D,
@@ -769,39 +835,46 @@ extern "C" int gh_lsm_fwd(const void* H, const void* W, const void* index, int i
   if (N == 0) return GH_OK;
   if (!H || !W || !index || !logprobs || !workspace) return set_error(GH_EINVAL, "null pointer argument");
   if ((rc = check_aligned({H, W, kept, workspace}))) return rc;
-  if (kept && dtype != GH_BF16) return set_error(GH_EUNSUPPORTED, "only bf16 operands keep e^x");
-  if (kept && kept_bytes < kept_layout(N, V).total) return set_error(GH_EWORKSPACE, "kept buffer too small");
+  const KeptLayout K = kept_layout(N, V, dtype);
+  if (kept && kept_bytes < K.total) return set_error(GH_EWORKSPACE, "kept buffer too small");
   const FwdLayout L = fwd_layout(N, V, chunk_rows, kept != nullptr);
   if (workspace_bytes < L.total)
     return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
+  char* kp = static_cast<char*>(kept);
   const float sc2 = (float)(inv_temperature * kLog2ed);
   int* status = reinterpret_cast<int*>(ws + L.status);
-  if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
-  char* kp = static_cast<char*>(kept);
+  int* tgt = reinterpret_cast<int*>(kp && dtype == GH_F16 ? kp + K.tgt : ws + L.tgt);
+  if ((rc = targets(index, index_dtype, N, V, ignore_index, tgt, status, st))) return rc;
   if (dtype == GH_BF16) return lsm_fwd_run<__nv_bfloat16>(H, W, N, D, V, dtype, sc2, L, kp, logprobs, state, ws, st);
-  return lsm_fwd_run<__half>(H, W, N, D, V, dtype, sc2, L, nullptr, logprobs, state, ws, st);
+  return lsm_fwd_run<__half>(H, W, N, D, V, dtype, sc2, L, kp, logprobs, state, ws, st);
 }
 
 extern "C" int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V,
-                               int dtype, double inv_temperature, const void* kept, size_t kept_bytes,
-                               void* grad_input, void* grad_weight, void* workspace, size_t workspace_bytes,
-                               void* stream) {
+                               int dtype, double inv_temperature, int64_t chunk_rows, int fp32_grad_weight_accum,
+                               const void* kept, size_t kept_bytes, void* grad_input, void* grad_weight,
+                               void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_common(N, D, V, dtype, GH_I64, inv_temperature);
   if (rc) return rc;
-  if (dtype != GH_BF16) return set_error(GH_EUNSUPPORTED, "only bf16 operands keep e^x");
   if (N == 0) return GH_OK;
   if (!H || !W || !grad || !kept || !workspace) return set_error(GH_EINVAL, "null pointer argument");
   if ((rc = check_aligned({H, W, kept, grad_input, grad_weight, workspace}))) return rc;
-  if (kept_bytes < kept_layout(N, V).total) return set_error(GH_EWORKSPACE, "kept buffer too small");
-  const BwdLayout L = bwd_layout(N, D, V, N, true, true);
+  const KeptLayout K = kept_layout(N, V, dtype);
+  if (kept_bytes < K.total) return set_error(GH_EWORKSPACE, "kept buffer too small");
+  const BwdLayout L = bwd_layout(N, D, V, chunk_rows, dtype == GH_BF16, fp32_grad_weight_accum);
   if (workspace_bytes < L.total)
     return set_error(GH_EWORKSPACE, "workspace too small: %zu < %zu", workspace_bytes, L.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  return lsm_bwd_kept_run(H, W, grad, N, D, V, (float)inv_temperature, static_cast<const char*>(kept), grad_input,
-                          grad_weight, L, ws, st);
+  const char* kp = static_cast<const char*>(kept);
+  const float inv_t = (float)inv_temperature;
+  if (dtype == GH_BF16)
+    return lsm_bwd_kept_run(H, W, grad, N, D, V, inv_t, kp, grad_input, grad_weight, L, ws, st);
+  cudaMemsetAsync(ws + L.status, 0, sizeof(int), st);
+  return lsm_bwd_run<__half>(H, W, reinterpret_cast<const int*>(kp + K.tgt), reinterpret_cast<const float*>(kp + K.y),
+                             reinterpret_cast<const float*>(kp + K.lse2), grad, N, D, V, dtype, inv_t, 0.f, kp,
+                             grad_input, grad_weight, fp32_grad_weight_accum, L, ws, st);
 }
 
 extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* state,
@@ -824,10 +897,11 @@ extern "C" int gh_lsm_bwd(const void* H, const void* W, const void* index, int i
   const float sc2 = (float)(inv_temperature * kLog2ed);
   const float *lse2 = state, *logprobs = state + N;
   int* status = reinterpret_cast<int*>(ws + L.status);
-  if ((rc = targets(index, index_dtype, N, V, ignore_index, reinterpret_cast<int*>(ws + L.tgt), status, st))) return rc;
+  int* tgt = reinterpret_cast<int*>(ws + L.tgt);
+  if ((rc = targets(index, index_dtype, N, V, ignore_index, tgt, status, st))) return rc;
   if (dtype == GH_BF16)
-    return lsm_bwd_run<__nv_bfloat16>(H, W, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, grad_input, grad_weight,
-                                      fp32_grad_weight_accum, L, ws, st);
-  return lsm_bwd_run<__half>(H, W, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, grad_input, grad_weight,
-                             fp32_grad_weight_accum, L, ws, st);
+    return lsm_bwd_run<__nv_bfloat16>(H, W, tgt, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, nullptr, grad_input,
+                                      grad_weight, fp32_grad_weight_accum, L, ws, st);
+  return lsm_bwd_run<__half>(H, W, tgt, logprobs, lse2, grad, N, D, V, dtype, inv_t, sc2, nullptr, grad_input,
+                             grad_weight, fp32_grad_weight_accum, L, ws, st);
 }

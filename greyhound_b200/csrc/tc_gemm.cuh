@@ -109,7 +109,7 @@ struct Params {
   // the operand type) and are scaled by sc2 = log2(e) / temperature.
   const int* tgt;         // [M] target column, negative: none
   float sc2;
-  float* gmax;            // EPI_LSM_Q: [num_n][2][M] shift of the groups that qmode flags
+  float* gmax;            // EPI_LSM_Q: [num_n][2][M] shift of the groups that qmode flags (fp16: of all)
   const float* lse2;      // EPI_LSM_GRAD: [M] log-sum-exp in log2 units
   const float* rfac;      // EPI_LSM_GRAD: [M] factor of (onehot - p)
   const float* tval;      // EPI_LSM_GRAD: [M] value at the target column
@@ -793,7 +793,8 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           // exponentials). EPI_LSM_Q also stores q = e^x in 16 bits (one ex2
           // does both), as e^(x - shift) with the group's largest logit as the
           // shift where that lies outside the window: two roundings of e^x
-          // relative to itself, whatever the size of the logits. Without the
+          // relative to itself, whatever the size of the logits. fp16, whose
+          // exponent has no such window, shifts every group. Without the
           // store the sums are formed the same way, so that a scoring pass and
           // a training pass over the same rows agree in every bit (the ratio of
           // their probabilities is exactly 1).
@@ -808,13 +809,15 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               if (col_g + j < p.N) cmax = fmaxf(cmax, v[j]);
           }
           const float cml = cmax * p.sc2;
-          const bool out_of_window = !(cml <= kLsmQHi && (cml >= kLsmQLo || cml == kNegInf));  // NaN: out
-          const float shift = out_of_window ? cml : 0.f;
+          constexpr bool kShiftAll = AbType<T>::v == 0;
+          const bool shifted =
+              kShiftAll ? cml != kNegInf : !(cml <= kLsmQHi && (cml >= kLsmQLo || cml == kNegInf));  // NaN: shifted
+          const float shift = shifted ? cml : 0.f;
           if constexpr (EPI == EPI_LSM_Q) {
             if (row_ok && col_g < p.N) {
               const int64_t gi = ((int64_t)nt * 2 + g) * p.M + row;
-              p.qmode[gi] = out_of_window ? 1 : 0;
-              if (out_of_window) p.gmax[gi] = cml;
+              if (!kShiftAll) p.qmode[gi] = shifted ? 1 : 0;
+              if (kShiftAll || shifted) p.gmax[gi] = cml;
             }
           }
           if ((unsigned)t_rel < (unsigned)NV) {

@@ -67,15 +67,16 @@ def _chunk(N: int, D: int, V: int) -> int:
     return chunk_size_for(N, D, V, 2) if N > 0 else 1
 
 
-def kept_bytes(N: int, V: int) -> int:
+def kept_bytes(N: int, V: int, dtype: torch.dtype) -> int:
     """``gh_lsm_kept_bytes``, in arithmetic that symbolic sizes go through, too."""
-    return ((N * ((V + 7) // 8 * 8) * 2 + 255) // 256 + (4 * N + 255) // 256) * 256
+    rows = (4 * N + 255) // 256
+    beside = rows if dtype == torch.bfloat16 else (8 * N * ((V + 255) // 256) + 255) // 256 + 3 * rows
+    return ((N * ((V + 7) // 8 * 8) * 2 + 255) // 256 + beside) * 256
 
 
 def keeps_exponentials(inputs: Tensor, weight: Tensor) -> bool:
-    """Whether the forward stores e^x for the backward: bf16 (fp16's exponent
-    cannot hold it) and a buffer of at most 4 GiB."""
-    if inputs.ndim != 2 or weight.ndim != 2 or inputs.dtype != torch.bfloat16:
+    """Whether the forward stores e^x for the backward: a buffer of at most 4 GiB."""
+    if inputs.ndim != 2 or weight.ndim != 2:
         return False
     return inputs.shape[0] * ((weight.shape[0] + 7) // 8 * 8) * 2 <= _KEEP_BYTES
 
@@ -103,7 +104,7 @@ def linear_logprobs(
         _lib.raise_pending(dev, "linear_selective_log_softmax")
         out = torch.empty(N, dtype=torch.float32, device=dev)
         state = torch.empty(2, N, dtype=torch.float32, device=dev) if want_state else None
-        kept = torch.empty(kept_bytes(N, V), dtype=torch.uint8, device=dev) if keep else None
+        kept = torch.empty(kept_bytes(N, V, inputs.dtype), dtype=torch.uint8, device=dev) if keep else None
         if N == 0:
             return out, state, kept
         x, w, idx = _operand(inputs), _operand(weight), index.contiguous()
@@ -132,6 +133,7 @@ def linear_logprobs_backward_kept(
     kept: Tensor,
     grad: Tensor,
     temperature: float,
+    fp32_grad_weight_accum: bool,
     want_input: bool,
     want_weight: bool,
 ) -> tuple[Tensor | None, Tensor | None]:
@@ -147,10 +149,10 @@ def linear_logprobs_backward_kept(
         gw = torch.empty((V, D), dtype=weight.dtype, device=dev) if want_weight else None
         if N == 0:
             return gi, gw.zero_() if gw is not None else None
-        ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, N, 1, 1), dev)
+        chunk, code, fp32 = _chunk(N, D, V), _lib.dtype_code(x.dtype), int(fp32_grad_weight_accum)
+        ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, code, 1, fp32), dev)
         st = lib.gh_lsm_bwd_kept(
-            x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), 1.0 / float(temperature),
-            kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
+            x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, code, 1.0 / float(temperature), chunk, fp32, kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax backward")
         _lib.raise_on_status(ws, "linear_selective_log_softmax backward")
@@ -185,7 +187,8 @@ def linear_logprobs_backward(
         if N == 0:
             return gi, gw.zero_() if gw is not None else None
         chunk = _chunk(N, D, V)
-        ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, 0, int(fp32_grad_weight_accum)), dev)
+        ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, _lib.dtype_code(x.dtype), 0,
+                                                            int(fp32_grad_weight_accum)), dev)
         st = lib.gh_lsm_bwd(
             x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), state.data_ptr(),
             g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), int(ignore_index),

@@ -207,11 +207,10 @@ def chunked_linear_selective_log_softmax(
     gradient, and the next call on the device raises ``ValueError``.
 
     Differentiable (once) with respect to ``inputs`` and ``weight``, for any
-    gradient of the log-probabilities. bf16 operands with ``N * V * 2`` bytes
-    up to 4 GiB keep ``e^x`` from the forward for that; otherwise the backward
-    recomputes the logits in row chunks, summing the weight gradient over the
-    chunks in fp32 or, with ``grad_weight_accum_dtype="weight"``, in the
-    parameter's type.
+    gradient of the log-probabilities. Up to ``N * V * 2`` bytes of 4 GiB the
+    forward keeps ``e^x`` for that; otherwise the backward recomputes the logits
+    in row chunks. The weight gradient is summed over chunks in fp32 or, with
+    ``grad_weight_accum_dtype="weight"``, in the parameter's type.
     """
     _check_accum_dtype(grad_weight_accum_dtype)
     if inputs.ndim < 1 or index.shape != inputs.shape[:-1]:

@@ -83,7 +83,7 @@ def linear_selective_log_softmax_kept(
 
 @linear_selective_log_softmax_kept.register_fake
 def _(inputs, weight, index, ignore_index, temperature):
-    kept = torch.empty(kept_bytes(inputs.shape[0], weight.shape[0]), dtype=torch.uint8, device=inputs.device)
+    kept = torch.empty(kept_bytes(inputs.shape[0], weight.shape[0], inputs.dtype), dtype=torch.uint8, device=inputs.device)
     return _rows(inputs), kept
 
 
@@ -120,16 +120,19 @@ def linear_selective_log_softmax_kept_bwd(
     kept: Tensor,
     grad: Tensor,
     temperature: float,
+    fp32_grad_weight_accum: bool,
     want_input: bool,
     want_weight: bool,
 ) -> tuple[Tensor, Tensor]:
     """(grad_input [N, D], grad_weight [V, D]); an unwanted one is empty."""
-    gi, gw = linear_logprobs_backward_kept(inputs, weight, kept, grad, temperature, want_input, want_weight)
+    gi, gw = linear_logprobs_backward_kept(
+        inputs, weight, kept, grad, temperature, fp32_grad_weight_accum, want_input, want_weight
+    )
     return _present(gi, gw, inputs, weight)
 
 
 @linear_selective_log_softmax_kept_bwd.register_fake
-def _(inputs, weight, kept, grad, temperature, want_input, want_weight):
+def _(inputs, weight, kept, grad, temperature, fp32_grad_weight_accum, want_input, want_weight):
     return _grads(inputs, weight, want_input, want_weight)
 
 
@@ -150,7 +153,7 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
             if plain:
                 return linear_logprobs(inputs, weight, index, ignore_index, temperature)[0]
             return linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)[0]
-        ctx.temperature = temperature
+        ctx.temperature, ctx.fp32_accum = temperature, fp32_grad_weight_accum
         ctx.kept = keeps_exponentials(inputs, weight)
         if ctx.kept:
             if plain:
@@ -163,7 +166,7 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
             out, state, _ = linear_logprobs(inputs, weight, index, ignore_index, temperature, want_state=True)
         else:
             out, state = linear_selective_log_softmax(inputs, weight, index, ignore_index, temperature)
-        ctx.ignore_index, ctx.fp32_accum = ignore_index, fp32_grad_weight_accum
+        ctx.ignore_index = ignore_index
         ctx.save_for_backward(inputs, weight, index, state)
         return out
 
@@ -175,7 +178,7 @@ class ChunkedLinearSelectiveLogSoftmaxFunction(torch.autograd.Function):
             inputs, weight, kept = ctx.saved_tensors
             bwd = linear_logprobs_backward_kept if _lib.eager(grad) else linear_selective_log_softmax_kept_bwd
             gi, gw = bwd(
-                inputs, weight, kept, grad, ctx.temperature, want[0], want[1]
+                inputs, weight, kept, grad, ctx.temperature, ctx.fp32_accum, want[0], want[1]
             )
         else:
             inputs, weight, index, state = ctx.saved_tensors

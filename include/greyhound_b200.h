@@ -341,26 +341,27 @@ GH_API int gh_scale(const void* in, void* out, int64_t n, int dtype, const float
  *           GH_DEV_BAD_LABEL
  *   state   [2, N] log-sum-exp in log2 units, and the log-probabilities once
  *           more (optional; gh_lsm_bwd needs it)
- *   kept    optional (BF16), gh_lsm_kept_bytes(): e^x in 16 bits and the row
- *           factors, which gh_lsm_bwd_kept reads (any number of times)
+ *   kept    optional, gh_lsm_kept_bytes(): e^x in 16 bits and what belongs to
+ *           it, which gh_lsm_bwd_kept reads (any number of times)
  * The backward takes the gradient `grad` [N] (F32) of logprobs and writes
  * grad_input [N, D] and / or grad_weight [V, D] (NULL: not computed) in the
  * operand type: gh_lsm_bwd_kept with two GEMMs, gh_lsm_bwd by repeating the
- * logits GEMM chunk_rows rows at a time, summing grad_weight over the chunks
- * in fp32 or (fp32_grad_weight_accum = 0) in the operand type.
+ * logits GEMM. It, and fp16 in gh_lsm_bwd_kept, goes chunk_rows rows at a time,
+ * summing grad_weight over the chunks in fp32 or (fp32_grad_weight_accum = 0)
+ * in the operand type.
  * ------------------------------------------------------------------------ */
-GH_API size_t gh_lsm_kept_bytes(int64_t N, int64_t V);
+GH_API size_t gh_lsm_kept_bytes(int64_t N, int64_t V, int dtype);
 GH_API size_t gh_lsm_fwd_workspace_bytes(int64_t N, int64_t V, int64_t chunk_rows, int keep);
-GH_API size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t chunk_rows, int kept,
+GH_API size_t gh_lsm_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t chunk_rows, int dtype, int kept,
                                          int fp32_grad_weight_accum);
 GH_API int gh_lsm_fwd(const void* H, const void* W, const void* index, int index_dtype, int64_t N, int64_t D,
                       int64_t V, int dtype, int64_t ignore_index, double inv_temperature, int64_t chunk_rows,
                       float* logprobs, float* state, void* kept, size_t kept_bytes, void* workspace,
                       size_t workspace_bytes, void* stream);
 GH_API int gh_lsm_bwd_kept(const void* H, const void* W, const float* grad, int64_t N, int64_t D, int64_t V,
-                           int dtype, double inv_temperature, const void* kept, size_t kept_bytes,
-                           void* grad_input, void* grad_weight, void* workspace, size_t workspace_bytes,
-                           void* stream);
+                           int dtype, double inv_temperature, int64_t chunk_rows, int fp32_grad_weight_accum,
+                           const void* kept, size_t kept_bytes, void* grad_input, void* grad_weight,
+                           void* workspace, size_t workspace_bytes, void* stream);
 GH_API int gh_lsm_bwd(const void* H, const void* W, const void* index, int index_dtype, const float* state,
                       const float* grad, int64_t N, int64_t D, int64_t V, int dtype,
                       int64_t ignore_index, double inv_temperature, int64_t chunk_rows,

@@ -48,7 +48,7 @@ def test_c_entries_refuse_bad_arguments():
         return lib.gh_lsm_fwd(H, W, 8, idt, 4, D, 9, dtype, -100, inv_t, 4, 8, None, kept, kb, ws, wb, None)
 
     def kept_bwd(dtype=BFC, wb=1 << 30, H=16, gi=16, gw=16, kept=16, kb=1 << 20):
-        return lib.gh_lsm_bwd_kept(H, 16, 8, 4, 16, 9, dtype, 1.0, kept, kb, gi, gw, 16, wb, None)
+        return lib.gh_lsm_bwd_kept(H, 16, 8, 4, 16, 9, dtype, 1.0, 4, 1, kept, kb, gi, gw, 16, wb, None)
 
     def bwd(index=8, wb=1 << 30, W=16, gi=16):
         return lib.gh_lsm_bwd(16, W, index, I64, 8, 8, 4, 16, 9, BFC, -100, 1.0, 4, 1, gi, 16, 16, wb, None)
@@ -60,12 +60,13 @@ def test_c_entries_refuse_bad_arguments():
         (fwd(inv_t=0.0), ValueError),
         (fwd(wb=16), RuntimeError),
         (fwd(kept=16, kb=16), RuntimeError),
-        (fwd(dtype=F16, kept=16, kb=1 << 20), RuntimeError),
+        (fwd(dtype=F16, kept=16, kb=64), RuntimeError),
         (fwd(H=8), ValueError),
         (fwd(W=2), ValueError),
         (fwd(ws=8), ValueError),
         (fwd(H=None), ValueError),
-        (kept_bwd(dtype=F16), RuntimeError),
+        (kept_bwd(dtype=F16, kb=64), RuntimeError),
+        (kept_bwd(dtype=F16, wb=64), RuntimeError),
         (kept_bwd(wb=16), RuntimeError),
         (kept_bwd(kb=16), RuntimeError),
         (kept_bwd(H=8), ValueError),
@@ -85,7 +86,9 @@ def test_buffer_sizes():
     recomputed backward, do not grow with N * V."""
     lib = _lib.load()
     for n, v in ((1, 1), (7, 9), (64, 100), (65, 128256), (16384, 131072)):
-        assert kept_bytes(n, v) == lib.gh_lsm_kept_bytes(n, v)
-    assert lib.gh_lsm_kept_bytes(8192, 128256) < 8192 * 128256 * 2 + (1 << 20)
+        assert kept_bytes(n, v, torch.bfloat16) == lib.gh_lsm_kept_bytes(n, v, _lib.GH_BF16)
+        assert kept_bytes(n, v, torch.float16) == lib.gh_lsm_kept_bytes(n, v, _lib.GH_F16)
+    assert lib.gh_lsm_kept_bytes(8192, 128256, _lib.GH_F16) < 8192 * 128256 * 2 + (64 << 20)
+    assert lib.gh_lsm_kept_bytes(8192, 128256, _lib.GH_BF16) < 8192 * 128256 * 2 + (1 << 20)
     assert lib.gh_lsm_fwd_workspace_bytes(65536, 128256, 8192, 0) < 64 << 20
-    assert lib.gh_lsm_bwd_workspace_bytes(65536, 4096, 128256, 8192, 0, 1) < (2 << 30) + 4 * 4096 * 128256 + (256 << 20)
+    assert lib.gh_lsm_bwd_workspace_bytes(65536, 4096, 128256, 8192, _lib.GH_BF16, 0, 1) < (2 << 30) + 4 * 4096 * 128256 + (256 << 20)

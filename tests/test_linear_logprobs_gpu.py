@@ -14,6 +14,9 @@ Tolerances (u = 2^-8 for bf16, 2^-11 for fp16, relative):
  * underflow: e^x below 2^-126 counts as 0 (ex2.ftz), and a row stored as e^x
    has a log-sum-exp of at least 2^-64, so a probability may be off by
    2^-126 / 2^-64 = 2^-62 absolutely: 2^-62 |g| sum |H| (or |W|) in the gradients.
+   fp16 stores e^x relative to the largest of 128, to a step of 2^-24, and the
+   gradient times at least 2^13 / max |g|, to the same step: 2^-25 of a
+   probability's largest neighbour and 2^-37 of the largest gradient.
 """
 
 import math
@@ -62,8 +65,12 @@ def definition(H, W, t, g, temperature=1.0):
     a = 3 * u * d.abs() + ey * g.abs() * lp.exp()
     bH = a @ W.abs() + 2 * u * dH.abs() + 2.0**-62 * g.abs() * W.abs().sum(0)
     bW = a.T @ H.abs() + 2 * u * dW.abs() + 2.0**-62 * (g.abs() * H.abs()).sum(0)
-    tiny = 2.0**-24 if u == 2.0**-11 else 0.0  # fp16's spacing near zero, of the results
-    return y, dH, dW, ey, bH + tiny, bW + tiny
+    if u == 2.0**-11:  # fp16's spacing near zero: of what is stored, and of the results
+        V = x.shape[1]
+        top = torch.nn.functional.pad(lp.exp(), (0, -V % 128)).view(len(x), -1, 128).amax(2).repeat_interleave(128, 1)[:, :V]
+        e = 2.0**-25 * g.abs() * top + 2.0**-37 * g.abs().amax()
+        bH, bW = bH + e @ W.abs() + 2.0**-24, bW + e.T @ H.abs() + 2.0**-24
+    return y, dH, dW, ey, bH, bW
 
 
 def check(H, W, t, g, temperature=1.0, **kw):
@@ -101,12 +108,12 @@ def test_temperature(dtype, temperature):
 
 @requires_gpu
 @pytest.mark.parametrize("accum", ["fp32", "weight"])
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_recomputed_backward_over_several_chunks(monkeypatch, dtype, accum):
+@pytest.mark.parametrize("dtype,keep", [(torch.bfloat16, False), (torch.float16, False), (torch.float16, True)])
+def test_backward_over_several_chunks(monkeypatch, dtype, keep, accum):
     """Chunks of 128 rows, the last one short: with fp32 accumulation the same
     bound; in the operand type each of the 4 partial sums is rounded (u each,
     relative to a partial sum of at most the sum of absolute terms)."""
-    monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    monkeypatch.setattr(K, "_KEEP_BYTES", K._KEEP_BYTES if keep else 0)
     monkeypatch.setattr(K, "_chunk", lambda N, D, V: 128)
     H, W, t, g = make(400, 128, 1111, dtype, 9, scale=2.0)
     if accum == "fp32":
@@ -120,19 +127,21 @@ def test_recomputed_backward_over_several_chunks(monkeypatch, dtype, accum):
 
 
 @requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("scale", [30.0, 120.0])
-def test_logits_outside_the_exponent_window(scale):
-    """Largest logits of about 100 and 400 (the stored e^x covers +-44): rows
+def test_logits_outside_the_exponent_window(scale, dtype):
+    """Largest logits of about 100 and 400 (e^x as stored in bf16 covers +-44): rows
     are rewritten, with the same bound; p_t near 1 and near 0 both occur."""
-    H, W, t, g = make(160, 64, 900, torch.bfloat16, 3, scale=scale)
+    H, W, t, g = make(160, 64, 900, dtype, 3, scale=scale)
     t[::2] = (H[::2].double() @ W.double().T).argmax(1)
     check(H, W, t, g)
 
 
 @requires_gpu
-def test_rows_of_very_small_and_shifted_logits():
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_of_very_small_and_shifted_logits(dtype):
     """Every logit of a row near -400 (below the window), beside normal rows."""
-    H, W, t, g = make(130, 64, 700, torch.bfloat16, 4)
+    H, W, t, g = make(130, 64, 700, dtype, 4)
     W[:, 0] = 20.0
     H[:, 0] = 0.0
     H[::3, 0] = -20.0
@@ -153,14 +162,15 @@ def test_confident_targets_keep_their_gradient():
 
 
 @requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("kept", [True, False])
-def test_left_out_rows_may_hold_anything(monkeypatch, kept):
+def test_left_out_rows_may_hold_anything(monkeypatch, kept, dtype):
     if not kept:
         monkeypatch.setattr(K, "_KEEP_BYTES", 0)
-    H, W, t, g = make(200, 64, 300, torch.bfloat16, 8)
+    H, W, t, g = make(200, 64, 300, dtype, 8)
     t[5], t[77], t[199] = -100, -100, -100
     clean = check(H, W, t, g)
-    H[5], H[77, 3], H[199] = float("nan"), float("inf"), 3e38
+    H[5], H[77, 3], H[199] = float("nan"), float("inf"), torch.finfo(dtype).max
     g[5], g[77] = float("nan"), float("inf")
     h, w = H.requires_grad_(True), W.requires_grad_(True)
     y = chunked_linear_selective_log_softmax(h, w, t)
@@ -169,8 +179,9 @@ def test_left_out_rows_may_hold_anything(monkeypatch, kept):
 
 
 @requires_gpu
-def test_nan_rows_stay_their_own():
-    H, W, t, g = make(70, 64, 300, torch.bfloat16, 8, left_out=0.0)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_nan_rows_stay_their_own(dtype):
+    H, W, t, g = make(70, 64, 300, dtype, 8, left_out=0.0)
     clean = check(H, W, t, g)
     H[9, 1] = float("nan")
     h = H.requires_grad_(True)
@@ -182,8 +193,9 @@ def test_nan_rows_stay_their_own():
 
 
 @requires_gpu
-def test_one_gradient_alone_and_no_gradient():
-    H, W, t, g = make(150, 128, 1000, torch.bfloat16, 11)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_gradient_alone_and_no_gradient(dtype):
+    H, W, t, g = make(150, 128, 1000, dtype, 11)
     y, dh, dw = check(H, W, t, g)
     assert torch.equal(chunked_linear_selective_log_softmax(H, W, t), y.detach())
     for keep in (K._KEEP_BYTES, 0):
@@ -200,10 +212,11 @@ def test_one_gradient_alone_and_no_gradient():
 
 
 @requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("scale", [1.0, 100.0])
-def test_scoring_and_training_forwards_agree_in_every_bit(monkeypatch, scale):
+def test_scoring_and_training_forwards_agree_in_every_bit(monkeypatch, scale, dtype):
     """The policy's ratio against log-probabilities taken without a gradient is exactly 1."""
-    H, W, t, g = make(300, 192, 1500, torch.bfloat16, 21, scale=scale)
+    H, W, t, g = make(300, 192, 1500, dtype, 21, scale=scale)
     scored = chunked_linear_selective_log_softmax(H, W, t)
     h = H.clone().requires_grad_(True)
     assert torch.equal(chunked_linear_selective_log_softmax(h, W, t).detach(), scored)
@@ -313,7 +326,7 @@ def test_opcheck():
     _, state = linear_selective_log_softmax(H, W, t, -100, 1.0)
     opcheck(linear_selective_log_softmax_bwd, (H, W, t, state, g, -100, 1.0, True, True, False))
     _, kept = linear_selective_log_softmax_kept(H, W, t, -100, 1.0)
-    opcheck(linear_selective_log_softmax_kept_bwd, (H, W, kept, g, 1.0, True, True))
+    opcheck(linear_selective_log_softmax_kept_bwd, (H, W, kept, g, 1.0, True, True, True))
 
 
 @requires_gpu
