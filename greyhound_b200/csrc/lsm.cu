@@ -325,15 +325,25 @@ lsm_gscale_kernel(const float* __restrict__ g, const int* __restrict__ tgt, int6
   }
 }
 
-// Row factor and target value of d for all rows.
+// Row factor and target value of d for all rows. As in the kept bf16 form the
+// target's entry shall not lose its row a rounding: the row is scaled by
+// (rounded / exact) entry, and arow, its inverse, goes into dH's epilogue and dW's
+// copy of H.
+template <typename T>
 __global__ void __launch_bounds__(256)
 lsm_factor_kernel(const float* __restrict__ g, const float* __restrict__ y, const int* __restrict__ tgt, float inv_t,
-                  const float* __restrict__ scale, int64_t rows, float* __restrict__ rfac, float* __restrict__ tval) {
+                  const float* __restrict__ scale, int64_t rows, float* __restrict__ rfac, float* __restrict__ tval,
+                  float* __restrict__ arow) {
   const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (r >= rows) return;
-  const float f = tgt[r] >= 0 ? g[r] * inv_t * (scale ? scale[0] : 1.f) : 0.f;
-  rfac[r] = f;
-  tval[r] = tgt[r] >= 0 ? -f * expm1f(y[r]) : 0.f;
+  const bool on = tgt[r] >= 0;
+  const float f = on ? g[r] * inv_t * (scale ? scale[0] : 1.f) : 0.f;
+  const float tv = on ? -f * expm1f(y[r]) : 0.f;
+  const float c = Elt<T>::to_f(Elt<T>::from_f(tv));
+  const bool fit = c != 0.f && fabsf(c) <= 3.4e38f && fabsf(tv) >= 1e-30f;  // neither 0, inf nor NaN
+  rfac[r] = fit ? f * (c / tv) : f;
+  tval[r] = fit ? c : tv;
+  arow[r] = !on ? 0.f : fit ? tv / c : 1.f;
 }
 
 // Backward, kept form in fp16: d = rfac (onehot - q 2^(shift - lse2)), 8 columns
@@ -372,14 +382,29 @@ lsm_unpack_kernel(const __half* __restrict__ q, int64_t ldq, const float* __rest
   }
 }
 
-// H with left-out rows zeroed (0 * NaN must not reach dW): the dW GEMM's second
-// operand where d is written out.
+// arow * H with left-out rows zeroed (0 * NaN must not reach dW): the dW GEMM's
+// second operand where d is written out.
+template <typename T>
 __global__ void __launch_bounds__(256)
-lsm_clean_rows_kernel(const uint4* __restrict__ H, const int* __restrict__ tgt, int64_t rows, int64_t vpr,
-                      uint4* __restrict__ out) {
+lsm_clean_rows_kernel(const T* __restrict__ H, const int* __restrict__ tgt, const float* __restrict__ arow,
+                      int64_t rows, int64_t vpr, T* __restrict__ out) {
   const int64_t n = rows * vpr;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    st16(out + i, tgt[i / vpr] >= 0 ? ld16(H + i) : make_uint4(0, 0, 0, 0));
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / vpr;
+    Vec16<T> v;
+    if (tgt[r] < 0) {
+      v.raw = make_uint4(0, 0, 0, 0);
+    } else {
+      v.raw = ld16(reinterpret_cast<const uint4*>(H) + i);
+      const float a = arow[r];
+      float f[8];
+      v.to_float(f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= a;
+      v.from_float(f);
+    }
+    st16(reinterpret_cast<uint4*>(out) + i, v.raw);
+  }
 }
 
 // out = row[r] * scale * sum_s part[s][r][c], the slices of a split-K product.
@@ -528,7 +553,7 @@ KeptLayout kept_layout(int64_t N, int64_t V, int dtype) {
 }
 
 struct BwdLayout {
-  size_t status = 0, scale = 64, tgt, rfac, tval, d, hs, dh2, acc, total;
+  size_t status = 0, scale = 64, tgt, rfac, tval, arow, d, hs, dh2, acc, total;
   int64_t chunk, ldd;
   bool need_acc;
 };
@@ -542,6 +567,7 @@ BwdLayout bwd_layout(int64_t N, int64_t D, int64_t V, int64_t chunk, bool kept, 
   L.tgt = off;  off = al256(off + (kept ? 0 : sizeof(int) * N));
   L.rfac = off; off = al256(off + sizeof(float) * N);  // kept: a
   L.tval = off; off = al256(off + (kept ? 0 : sizeof(float) * N));
+  L.arow = off; off = al256(off + (kept ? 0 : sizeof(float) * N));
   L.d = off;    off = al256(off + (kept ? 0 : (size_t)chunk * L.ldd * 2));
   L.hs = off;   off = al256(off + (size_t)chunk * D * 2);
   // the last chunk may be shorter and take more slices of fewer rows
@@ -735,6 +761,7 @@ int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, co
   const KeptLayout K = kept_layout(N, V, dtype);
   float* rfac = reinterpret_cast<float*>(ws + L.rfac);
   float* tval = reinterpret_cast<float*>(ws + L.tval);
+  float* arow = reinterpret_cast<float*>(ws + L.arow);
   float* acc = reinterpret_cast<float*>(ws + L.acc);
   T* d = reinterpret_cast<T*>(ws + L.d);
   T* hs = reinterpret_cast<T*>(ws + L.hs);
@@ -746,7 +773,7 @@ int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, co
     count_launch(1);
     scale = s;
   }
-  lsm_factor_kernel<<<(unsigned)((N + 255) / 256), 256, 0, st>>>(grad, y, tgt, inv_t, scale, N, rfac, tval);
+  lsm_factor_kernel<T><<<(unsigned)((N + 255) / 256), 256, 0, st>>>(grad, y, tgt, inv_t, scale, N, rfac, tval, arow);
   count_launch(1);
   int rc = check_launch("lsm_factor");
   if (rc) return rc;
@@ -780,8 +807,7 @@ int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, co
       if ((rc = logits_gemm<T, gemm::EPI_LSM_GRAD>(Hc, W, rows, D, V, dtype, p, st))) return rc;
     }
     if (dW) {
-      lsm_clean_rows_kernel<<<4 * sms, 256, 0, st>>>(reinterpret_cast<const uint4*>(Hc), tgt + s0, rows, D / 8,
-                                                     reinterpret_cast<uint4*>(hs));
+      lsm_clean_rows_kernel<T><<<4 * sms, 256, 0, st>>>(Hc, tgt + s0, arow + s0, rows, D / 8, hs);
       count_launch(1);
       if ((rc = check_launch("lsm_clean_rows"))) return rc;
       void* out = dW;
@@ -800,7 +826,7 @@ int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, co
         return rc;
     }
     if (dH && (rc = dh_gemm<T>(dtype, Operand{d, L.ldd, 0}, W, rows, D, V, static_cast<T*>(dH) + s0 * D, unscale,
-                               nullptr, ws + L.dh2, status, nullptr, st)))
+                               arow + s0, ws + L.dh2, status, nullptr, st)))
       return rc;
   }
   return publish_status(status, st);
