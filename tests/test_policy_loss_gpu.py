@@ -312,3 +312,21 @@ def test_without_gradients():
     with torch.no_grad():
         got = clipped_policy_loss(lp, b["old"], b["adv"], mask=b["mask"], cu_seqlens=b["cu"], clip_high=0.3)
     assert torch.equal(got, loss) and not got.requires_grad
+
+
+@requires_gpu
+def test_more_than_2_to_the_31_tokens():
+    """Ratio 1 everywhere: the loss is minus the advantages' mean, weighted by length, and so is the gradient."""
+    T = (1 << 31) + 777
+    lp = torch.full((T,), -1.0, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    cu = torch.tensor([0, 100, (1 << 31) + 5, T - 7], device="cuda")
+    adv = torch.tensor([1.0, 2.0, -4.0], device="cuda")
+    n = [100, (1 << 31) - 95, 765]
+    total = sum(n)
+    loss, metrics = clipped_policy_loss(lp, lp.detach(), adv, cu_seqlens=cu, reduction="sum", return_metrics=True)
+    want = -(n[0] * 1.0 + n[1] * 2.0 - n[2] * 4.0)
+    assert abs(loss.item() - want) <= 2 * F * abs(want)
+    assert abs(metrics.tokens.item() - total) <= 2 * F * total
+    (g,) = torch.autograd.grad(loss, lp)
+    assert g[0] == -1 and g[100] == -2 and g[(1 << 31) + 4] == -2 and g[(1 << 31) + 5] == 4
+    assert g[T - 8] == 4 and (g[T - 7 :] == 0).all() and (g[100 : (1 << 31) + 5 : 4099] == -2).all()

@@ -213,3 +213,18 @@ def test_captured_and_on_another_stream(lengths):
         out.zero_()
         graph.replay()
         assert torch.equal(out, grad)
+
+
+@requires_gpu
+def test_more_than_2_to_the_31_tokens():
+    """Sums of 2^31 equal differences, exact in fp64."""
+    T = (1 << 31) + 777
+    lp = torch.full((T,), -0.5, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    cu = torch.tensor([0, 1 << 10, T], device="cuda")
+    loss, rewards = preference_loss(lp, None, cu_seqlens=cu, beta=1.0, length_normalized=True, return_rewards=True)
+    assert rewards.chosen.item() == -0.5 and rewards.rejected.item() == -0.5
+    (g,) = torch.autograd.grad(loss, lp)
+    assert g[0].item() == -0.5 / 1024 and g[1023] == g[0]
+    want = 0.5 / (T - 1024)
+    for i in (1024, (1 << 31) - 1, 1 << 31, T - 1):
+        assert abs(g[i].item() - want) <= 2.0**-8 * want
