@@ -125,7 +125,8 @@ __device__ __forceinline__ void block_totals(double (&v)[K], double (*scratch)[3
 // One sequence's (or warp's) sums.
 struct Sums {
   double loss, kl;
-  int clipped, n;
+  int64_t n;
+  int clipped;  // of a warp's tokens at most
 };
 
 // ---------------------------------------------------------------------------
@@ -160,7 +161,7 @@ enum { RED_SUM = 0, RED_MEAN = 1, RED_SEQ_MEAN = 2 };
 struct PolicyOut {
   float *loss, *metrics;  // metrics: mean kl, share of clipped tokens, tokens
   float* scal;
-  Sums *warps, *slots, *seqs;
+  Sums *parts, *slots, *seqs;  // a block's (or, in the one block, a warp's) sums; (warp, sequence)'s; sequences'
 };
 
 // e^u - 1 and e^u - 1 - u. Differences of e^u would cancel at small u: the second
@@ -183,24 +184,26 @@ __device__ __forceinline__ float kl_terms(float u, float& em1) {
   return small ? near : far - u;
 }
 
-// The warp's tokens [t0, t1): gradients, one Sums per part (want_slots) and
+// The warp's tokens [t0, t1): gradients, one Sums per part (want_slots); returns
 // the warp's own.
 template <typename T, typename R, bool KL>
-__device__ __forceinline__ void policy_tokens(const Seqs& q, const Policy& p, int64_t w, int64_t span, bool want_slots,
+__device__ __forceinline__ Sums policy_tokens(const Seqs& q, const Policy& p, int64_t w, int64_t span, bool want_slots,
                                               const PolicyOut& o) {
   const int lane = threadIdx.x & 31;
   const T* lp = static_cast<const T*>(p.lp);
   const R* old = static_cast<const R*>(p.old);
   const R* ref = static_cast<const R*>(p.ref);
   const int64_t t0 = w * span, t1 = t0 + span < q.T ? t0 + span : q.T;
-  Sums all{0.0, 0.0, 0, 0};
+  double all_loss = 0.0, all_kl = 0.0;
+  int all_clipped = 0, all_n = 0;  // of a span
   walk(q, t0, t1, [&](int64_t s, int64_t a, int64_t b) {
     if (s < 0) {
       if (p.d)
         for (int64_t t = a + lane; t < b; t += 32) p.d[t] = 0.f;
       return;
     }
-    Sums sum{0.0, 0.0, 0, 0};
+    double loss = 0.0, kl = 0.0;
+    int clipped = 0, valid = 0;
     // 32-bit offsets from the part's first token (a part is at most a span).
     // What is absent is read with stride 0 from an address that is there: no
     // branch stands between a lane's loads, and none of them waits for the mask.
@@ -267,66 +270,65 @@ __device__ __forceinline__ void policy_tokens(const Seqs& q, const Policy& p, in
             k4 += k3;
           }
           l4 += l;
-          sum.clipped += above || below;
-          sum.n += 1;
+          clipped += above || below;
+          ++valid;
         }
         if (da && t + 32 * j < n) da[t + 32 * j] = g;
       }
-      sum.loss += (double)l4;
-      if (KL) sum.kl += (double)k4;
+      loss += (double)l4;
+      if (KL) kl += (double)k4;
     }
-    sum.loss = warp_sum(sum.loss);
-    if (KL) sum.kl = warp_sum(sum.kl);
-    sum.clipped = warp_sum(sum.clipped);
-    sum.n = warp_sum(sum.n);
-    if (want_slots && lane == 0) o.slots[w + s] = sum;
-    all.loss += sum.loss;
-    all.kl += sum.kl;
-    all.clipped += sum.clipped;
-    all.n += sum.n;
+    loss = warp_sum(loss);
+    if (KL) kl = warp_sum(kl);
+    clipped = warp_sum(clipped);
+    valid = warp_sum(valid);
+    if (want_slots && lane == 0) o.slots[w + s] = Sums{loss, kl, valid, clipped};
+    all_loss += loss;
+    all_kl += kl;
+    all_clipped += clipped;
+    all_n += valid;
   });
-  if (lane == 0) o.warps[w] = all;
+  return Sums{all_loss, all_kl, all_n, all_clipped};
 }
 
 // Sequence s from its slots, by one warp; lane 0 writes it.
 __device__ __forceinline__ void policy_sequence(const Seqs& q, int64_t s, int64_t span, const PolicyOut& o) {
   const int lane = threadIdx.x & 31;
   const int64_t a = seq_start(q, s), b = seq_start(q, s + 1);
-  Sums sum{0.0, 0.0, 0, 0};
+  Sums sum{};
+  double n = 0.0;
   if (b > a)
     for (int64_t w = a / span + lane; w <= (b - 1) / span; w += 32) {
       const Sums& x = o.slots[w + s];
       sum.loss += x.loss;
-      sum.n += x.n;
+      n += (double)x.n;
     }
   sum.loss = warp_sum(sum.loss);
-  sum.n = warp_sum(sum.n);
+  sum.n = (int64_t)warp_sum(n);
   if (lane == 0) o.seqs[s] = sum;
 }
 
 // The last step, by one block.
-__device__ __forceinline__ void policy_total(const Seqs& q, int64_t warps, int red, const PolicyOut& o) {
+__device__ __forceinline__ void policy_total(const Seqs& q, int64_t parts, int red, const PolicyOut& o) {
   __shared__ double scratch[5][32];
-  Sums all{0.0, 0.0, 0, 0};
-  for (int64_t w = threadIdx.x; w < warps; w += blockDim.x) {
-    const Sums x = o.warps[w];
-    all.loss += x.loss;
-    all.kl += x.kl;
-    all.clipped += x.clipped;
-    all.n += x.n;
+  double loss = 0.0, kl_sum = 0.0, clipped_sum = 0.0, n_sum = 0.0;  // counts in fp64: exact up to 2^53
+  for (int64_t w = threadIdx.x; w < parts; w += blockDim.x) {
+    const Sums x = o.parts[w];
+    loss += x.loss;
+    kl_sum += x.kl;
+    clipped_sum += (double)x.clipped;
+    n_sum += (double)x.n;
   }
-  double loss = all.loss;
   int filled = 0;
   if (red == RED_SEQ_MEAN) {
     loss = 0.0;
     for (int64_t s = threadIdx.x; s < q.S; s += blockDim.x) {
       const Sums x = o.seqs[s];
-      if (x.n > 0) loss += x.loss / x.n;
+      if (x.n > 0) loss += x.loss / (double)x.n;
       filled += x.n > 0;
     }
   }
-  // counts in fp64: exact, and a batch may hold more than 2^31 tokens
-  double v[5] = {loss, all.kl, (double)all.clipped, (double)all.n, (double)filled};
+  double v[5] = {loss, kl_sum, clipped_sum, n_sum, (double)filled};
   block_totals(v, scratch);
   if (threadIdx.x == 0) {
     loss = v[0];
@@ -343,19 +345,33 @@ __device__ __forceinline__ void policy_total(const Seqs& q, int64_t warps, int r
   }
 }
 
+// Four blocks an SM, so that the 32 warps an SM that cut_tokens makes run at once.
 template <typename T, typename R, bool KL>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __launch_bounds__(32 * kWarps, 4)
 policy_tokens_kernel(Seqs q, Policy p, int64_t warps, int64_t span, int want_slots, PolicyOut o) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   check_offsets(q, i, (int64_t)gridDim.x * blockDim.x);
-  if (i / 32 < warps) policy_tokens<T, R, KL>(q, p, i / 32, span, want_slots, o);
+  __shared__ Sums sums[kWarps];
+  Sums mine{};
+  if (i / 32 < warps) mine = policy_tokens<T, R, KL>(q, p, i / 32, span, want_slots, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < kWarps; ++k) {
+      mine.loss += sums[k].loss;
+      mine.kl += sums[k].kl;
+      mine.n += sums[k].n;
+      mine.clipped += sums[k].clipped;
+    }
+    o.parts[blockIdx.x] = mine;
+  }
 }
 __global__ void __launch_bounds__(32 * kWarps) policy_sequences_kernel(Seqs q, int64_t span, PolicyOut o) {
   const int64_t s = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
   if (s < q.S) policy_sequence(q, s, span, o);
 }
-__global__ void __launch_bounds__(1024) policy_total_kernel(Seqs q, int64_t warps, int red, PolicyOut o) {
-  policy_total(q, warps, red, o);
+__global__ void __launch_bounds__(1024) policy_total_kernel(Seqs q, int64_t parts, int red, PolicyOut o) {
+  policy_total(q, parts, red, o);
 }
 // Everything in one block.
 template <typename T, typename R, bool KL>
@@ -363,7 +379,10 @@ __global__ void __launch_bounds__(32 * kOneWarps)
 policy_one_kernel(Seqs q, Policy p, int64_t warps, int64_t span, int red, PolicyOut o) {
   check_offsets(q, threadIdx.x, blockDim.x);
   const int64_t w = threadIdx.x >> 5;
-  if (w < warps) policy_tokens<T, R, KL>(q, p, w, span, red == RED_SEQ_MEAN, o);
+  if (w < warps) {
+    const Sums mine = policy_tokens<T, R, KL>(q, p, w, span, red == RED_SEQ_MEAN, o);
+    if ((threadIdx.x & 31) == 0) o.parts[w] = mine;
+  }
   __syncthreads();
   if (red == RED_SEQ_MEAN) {
     for (int64_t s = w; s < q.S; s += blockDim.x >> 5) policy_sequence(q, s, span, o);
@@ -402,7 +421,7 @@ policy_bwd_kernel(Seqs q, const float* __restrict__ d, const float* __restrict__
     return;
   }
   walk(q, t0, t1, [&](int64_t s, int64_t a, int64_t b) {
-    const int n = s >= 0 ? seqs[s].n : 0;
+    const int64_t n = s >= 0 ? seqs[s].n : 0;
     part(n > 0 ? c / (float)n : 0.f, a, b);
   });
 }
@@ -620,14 +639,14 @@ Cut cut_tokens(int64_t T, int64_t S, bool may_be_one) {
 }
 
 struct PolicyLayout {
-  size_t seqs, warps, slots, total;
+  size_t seqs, parts, slots, total;
 };
 PolicyLayout policy_layout(int64_t T, int64_t S, int red) {
   const Cut c = cut_tokens(T, S, true);
   PolicyLayout L;
   size_t off = 0;
   L.seqs = off;  off = al256(off + (red == RED_SEQ_MEAN ? sizeof(Sums) * (size_t)S : 0));
-  L.warps = off; off = al256(off + sizeof(Sums) * (size_t)c.warps);
+  L.parts = off; off = al256(off + sizeof(Sums) * (size_t)(c.one ? kOneWarps : c.warps / kWarps + 1));
   L.slots = off; off = al256(off + (red == RED_SEQ_MEAN ? sizeof(Sums) * (size_t)(c.warps + S) : 0));
   L.total = off;
   return L;
@@ -681,7 +700,7 @@ int launch_policy(const Seqs& q, const Policy& p, int red, const PolicyOut& o, c
     policy_sequences_kernel<<<blocks_of(q.S), 32 * kWarps, 0, st>>>(q, c.span, o);
     count_launch(1);
   }
-  policy_total_kernel<<<1, 1024, 0, st>>>(q, c.warps, red, o);
+  policy_total_kernel<<<1, 1024, 0, st>>>(q, grid, red, o);
   return check_launch("gh_policy_loss_fwd");
 }
 
@@ -772,7 +791,7 @@ extern "C" int gh_policy_loss_fwd(const void* logprobs, int dtype, const void* o
   o.loss = loss;
   o.metrics = metrics;
   o.scal = scal;
-  o.warps = reinterpret_cast<Sums*>(ws + L.warps);
+  o.parts = reinterpret_cast<Sums*>(ws + L.parts);
   o.slots = reinterpret_cast<Sums*>(ws + L.slots);
   o.seqs = reinterpret_cast<Sums*>(ws + L.seqs);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

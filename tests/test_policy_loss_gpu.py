@@ -329,4 +329,7 @@ def test_more_than_2_to_the_31_tokens():
     assert abs(metrics.tokens.item() - total) <= 2 * F * total
     (g,) = torch.autograd.grad(loss, lp)
     assert g[0] == -1 and g[100] == -2 and g[(1 << 31) + 4] == -2 and g[(1 << 31) + 5] == 4
+    mean = clipped_policy_loss(lp, None, torch.full((1,), 3.0, device="cuda"), reduction="sequence_mean")  # one sequence
+    assert abs(mean.item() + 3.0) <= 8 * F
+    assert abs(torch.autograd.grad(mean, lp)[0][T - 1].item() + 3.0 / T) <= 2.0**-8 * 3.0 / T
     assert g[T - 8] == 4 and (g[T - 7 :] == 0).all() and (g[100 : (1 << 31) + 5 : 4099] == -2).all()
