@@ -120,6 +120,10 @@ def clip_tensors(
         norm = torch.empty((), dtype=torch.float32, device=device)
         ws = _lib.workspace(lib.gh_global_norm_workspace_bytes(n), device)
         ins = array("Q", map(Tensor.data_ptr, src))
+        if 0 in ins:  # empty ones, or wrappers around other tensors
+            for i, t in enumerate(src):
+                if ins[i] == 0 and t.numel() > 0:
+                    raise TypeError(f"tensor {i} ({type(t).__name__}) has no memory of its own; pass its local tensor")
         outs = None if dst is None else ins if dst is src else array("Q", map(Tensor.data_ptr, dst))
         sizes = array("q", map(Tensor.numel, src))
         st = lib.gh_clip_by_global_norm(

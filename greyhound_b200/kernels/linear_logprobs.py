@@ -152,7 +152,9 @@ def linear_logprobs_backward_kept(
         chunk, code, fp32 = _chunk(N, D, V), _lib.dtype_code(x.dtype), int(fp32_grad_weight_accum)
         ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, code, 1, fp32), dev)
         st = lib.gh_lsm_bwd_kept(
-            x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, code, 1.0 / float(temperature), chunk, fp32, kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
+            x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, code, 1.0 / float(temperature), chunk, fp32,
+            kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(),
+            _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax backward")
         _lib.raise_on_status(ws, "linear_selective_log_softmax backward")

@@ -258,7 +258,8 @@ def preference_loss_forward(
         st = lib.gh_preference_loss_fwd(
             lp.data_ptr(), _lib.dtype_code(lp.dtype), _lib.ptr(ref), other, _lib.ptr(m), lay.tokens,
             _lib.ptr(lay.cu), lay.cu_code, lay.seqs, float(beta), float(margin), float(label_smoothing),
-            KINDS[loss_type], int(length_normalized), int(reduction == "mean"), loss.data_ptr(), at, at + 4 * lay.seqs, ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
+            KINDS[loss_type], int(length_normalized), int(reduction == "mean"), loss.data_ptr(), at,
+            at + 4 * lay.seqs, ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
         )
         _lib.check(st, "preference_loss")
         _lib.raise_on_report(dev, "preference_loss")

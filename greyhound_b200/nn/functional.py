@@ -17,11 +17,11 @@ from typing import Any, Literal, NamedTuple, cast
 import torch
 from torch import Tensor
 
+from greyhound_b200.kernels.token_losses import _no_grad_to
 from greyhound_b200.ops.chunked_linear_cross_entropy import ChunkedLinearCrossEntropyFunction
 from greyhound_b200.ops.chunked_linear_loss import ChunkedLinearLossFunction
 from greyhound_b200.ops.chunked_linear_selective_log_softmax import ChunkedLinearSelectiveLogSoftmaxFunction
 from greyhound_b200.ops.cross_entropy import CrossEntropyFunction
-from greyhound_b200.kernels.token_losses import _no_grad_to
 from greyhound_b200.ops.logprobs import SelectiveLogSoftmaxFunction
 from greyhound_b200.ops.token_losses import ClippedPolicyLossFunction, PreferenceLossFunction
 

@@ -251,3 +251,36 @@ def test_autograd_notices_clipping_in_place():
         z.backward()
     with torch.inference_mode():
         clip_by_global_norm([y.clone()], 0.1, out=[torch.empty_like(y)])
+
+
+class _Wrapper(torch.Tensor):
+    """A tensor without memory of its own, as distributed ones are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+@requires_gpu
+def test_wrappers_around_other_tensors_are_refused():
+    t = torch.ones(8, device="cuda")
+    with pytest.raises((TypeError, RuntimeError)):
+        global_norm([t, _Wrapper(t)])
+    with pytest.raises((TypeError, RuntimeError)):
+        clip_by_global_norm([_Wrapper(t)], 1.0, out=[t])
+
+
+@requires_gpu
+def test_within_a_compiled_function():
+    ts = make([(300,), (17, 9)], TYPES, 12)
+    limit = 0.5 * norm64(ts)
+
+    def scaled(a, b):
+        (x, y), n = clip_by_global_norm([a + 0.0, b + 0.0], limit)
+        return x * 2, y * 2, n
+
+    for got, want in zip(torch.compile(scaled)(*ts), scaled(*ts)):
+        assert torch.equal(got, want)
