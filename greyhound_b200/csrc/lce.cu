@@ -83,6 +83,7 @@ int run_gemm(int dtype, const Operand& A, const Operand& B, int64_t M, int64_t N
   gemm::Params p{};
   set_tiles(p, M, N, K, pair, nsub, tl.ksplit);
   p.out2 = tl.ksplit > 1 ? split_out : nullptr;
+  p.k_wrap = (int)((A.wrap + BK - 1) / BK);
   p.raster = raster;
   p.group = 1;
   // tile-order override for the gradient GEMMs, "raster,group"

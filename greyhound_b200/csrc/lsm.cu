@@ -16,7 +16,8 @@
 //   kept       the forward's epilogue also stores q = e^x in 16 bits. In bf16, with
 //              a[r] = -g[r] / temperature * e^-lse[r], d = a (q - e^lse onehot):
 //              the one-hot part goes into q's target column, a into dH's epilogue
-//              and into a 16-bit copy of H for dW. Three GEMMs for both passes.
+//              and into a 16-bit copy of H for dW (up to 128 rows into two, the
+//              value and its rest). Three GEMMs for both passes.
 //              fp16's exponent cannot hold e^x: every 128-column group of a row is
 //              stored relative to its largest value, and a pass over a chunk of
 //              rows turns that into d.
@@ -24,6 +25,7 @@
 //              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, but 2 GB of
 //              workspace whatever N.
 // Bound by the tensor pipe for many rows and by reading W once for few.
+#include <algorithm>
 #include <initializer_list>
 
 #include "row_ops.cuh"
@@ -292,33 +294,47 @@ lsm_combine_kernel(const float2* __restrict__ stats, int num_n, int64_t rows, in
   }
 }
 
+// Eight elements of the dW GEMM's second operand, in 16 bits. With lo > 0, what
+// the rounding took off follows lo vectors further on.
+template <typename T>
+__device__ __forceinline__ void put_operand(T* hs, int64_t i, int64_t lo, const float (&f)[8]) {
+  Vec16<T> v;
+  v.from_float(f);
+  st16(reinterpret_cast<uint4*>(hs) + i, v.raw);
+  if (!lo) return;
+  float r[8], rest[8];
+  v.to_float(r);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) rest[k] = fabsf(r[k]) <= 3.4e38f ? f[k] - r[k] : 0.f;  // not inf - inf
+  v.from_float(rest);
+  st16(reinterpret_cast<uint4*>(hs) + lo + i, v.raw);
+}
+
 // Backward, kept form: a[r] = -g[r] / temperature * alpha0[r] and a * H in 16
 // bits, the dW GEMM's second operand (its rounding is dW's only one before
-// the output's). Left-out rows give exact zeros.
+// the output's, and pad > 0 leaves none: two parts of `pad` rows). Left-out rows
+// give exact zeros, as do those up to pad.
 __global__ void __launch_bounds__(256)
 lsm_rows_kernel(const __nv_bfloat16* __restrict__ H, const float* __restrict__ g, const float* __restrict__ alpha0,
-                float inv_t, int64_t rows, int64_t D, float* __restrict__ a_out, __nv_bfloat16* __restrict__ hs,
-                int* status) {
+                float inv_t, int64_t rows, int64_t pad, int64_t D, float* __restrict__ a_out,
+                __nv_bfloat16* __restrict__ hs, int* status) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;  // for the GEMMs that follow
-  const int64_t vpr = D / 8, n = rows * vpr;
+  const int64_t vpr = D / 8, n = (pad ? pad : rows) * vpr, lo = pad * vpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / vpr;
-    const float a0 = alpha0[r];
+    const float a0 = r < rows ? alpha0[r] : 0.f;
     const float a = a0 == 0.f ? 0.f : -g[r] * inv_t * a0;
-    if (i - r * vpr == 0) a_out[r] = a;
+    if (r < rows && i - r * vpr == 0) a_out[r] = a;
     if (!hs) continue;
-    Vec16<__nv_bfloat16> v;
-    if (a0 == 0.f) {
-      v.raw = make_uint4(0, 0, 0, 0);
-    } else {
+    float f[8] = {};
+    if (a0 != 0.f) {
+      Vec16<__nv_bfloat16> v;
       v.raw = ld16(reinterpret_cast<const uint4*>(H) + i);
-      float f[8];
       v.to_float(f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] *= a;
-      v.from_float(f);
     }
-    st16(reinterpret_cast<uint4*>(hs) + i, v.raw);
+    put_operand(hs, i, lo, f);
   }
 }
 
@@ -406,27 +422,24 @@ lsm_unpack_kernel(const __half* __restrict__ q, int64_t ldq, const float* __rest
 }
 
 // arow * H with left-out rows zeroed (0 * NaN must not reach dW): the dW GEMM's
-// second operand where d is written out.
+// second operand where d is written out; pad as above.
 template <typename T>
 __global__ void __launch_bounds__(256)
 lsm_clean_rows_kernel(const T* __restrict__ H, const int* __restrict__ tgt, const float* __restrict__ arow,
-                      int64_t rows, int64_t vpr, T* __restrict__ out) {
-  const int64_t n = rows * vpr;
+                      int64_t rows, int64_t pad, int64_t vpr, T* __restrict__ out) {
+  const int64_t n = (pad ? pad : rows) * vpr, lo = pad * vpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / vpr;
-    Vec16<T> v;
-    if (tgt[r] < 0) {
-      v.raw = make_uint4(0, 0, 0, 0);
-    } else {
+    float f[8] = {};
+    if (r < rows && tgt[r] >= 0) {
+      Vec16<T> v;
       v.raw = ld16(reinterpret_cast<const uint4*>(H) + i);
       const float a = arow[r];
-      float f[8];
       v.to_float(f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] *= a;
-      v.from_float(f);
     }
-    st16(reinterpret_cast<uint4*>(out) + i, v.raw);
+    put_operand(out, i, lo, f);
   }
 }
 
@@ -455,6 +468,16 @@ lsm_join_kernel(const float* __restrict__ part, int slices, int64_t n, int64_t D
 
 // ---------------------------------------------------------------------------
 // Host side
+
+// Rows of each part of the dW GEMM's second operand where it is taken in two
+// parts (value and rest, one after the other along K), else 0. Up to 128 rows the
+// product is bound by writing dW and a K twice as long costs little: 64 x 4096 x
+// 128256 705 -> 716 us a step, 128 x 1024 x 32000 91 -> 98, and dW is 1.66e-3 off
+// (its own rounding) instead of 2.35e-3; 256 x 4096 x 128256 would take 946 for 810.
+int64_t dw_pad(int64_t rows) { return rows <= 128 ? (rows + BK - 1) / BK * BK : 0; }
+// The dW product's K and first operand for `rows` rows of q or d.
+int64_t dw_k(int64_t rows) { return dw_pad(rows) ? 2 * dw_pad(rows) : rows; }
+Operand dw_operand(const void* d, int64_t ldd, int64_t rows) { return Operand{d, ldd, 1, dw_pad(rows) ? rows : 0}; }
 
 // K slices of the dH product [rows, D] over K = V. Its few output tiles leave
 // most SMs idle at a few hundred rows (512 x 1024 over 32000: 8 pair tiles for 74
@@ -592,9 +615,9 @@ BwdLayout bwd_layout(int64_t N, int64_t D, int64_t V, int64_t chunk, bool kept, 
   L.tval = off; off = al256(off + (kept ? 0 : sizeof(float) * N));
   L.arow = off; off = al256(off + (kept ? 0 : sizeof(float) * N));
   L.d = off;    off = al256(off + (kept ? 0 : (size_t)chunk * L.ldd * 2));
-  L.hs = off;   off = al256(off + (size_t)chunk * D * 2);
-  // the last chunk may be shorter and take more slices of fewer rows
+  // the last chunk may be shorter, be taken in two parts and in more slices of fewer rows
   const int64_t rest = N > 0 ? N - (N - 1) / chunk * chunk : 0;
+  L.hs = off;   off = al256(off + (size_t)std::max(dw_k(chunk), dw_k(rest)) * D * 2);
   const size_t a = dh_scratch(chunk, D, V), b = dh_scratch(rest, D, V);
   L.dh2 = off;  off = al256(off + (a > b ? a : b));
   L.need_acc = !kept && fp32_accum && N > chunk;
@@ -761,12 +784,12 @@ int lsm_bwd_kept_run(const void* H, const void* W, const float* grad, int64_t N,
   float* a = reinterpret_cast<float*>(ws + L.rfac);
   __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(ws + L.hs);
   lsm_rows_kernel<<<4 * sms, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(H), grad,
-                                           reinterpret_cast<const float*>(kept + K.alpha0), inv_t, N, D, a,
+                                           reinterpret_cast<const float*>(kept + K.alpha0), inv_t, N, dw_pad(N), D, a,
                                            dW ? hs : nullptr, status);
   count_launch(1);
   if ((rc = check_launch("lsm_rows"))) return rc;
-  if (dW && (rc = run_gemm(GH_BF16, Operand{kept + K.q, K.ldq, 1}, Operand{hs, D, 1}, V, D, N, dW, GH_BF16, D, nullptr,
-                           nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
+  if (dW && (rc = run_gemm(GH_BF16, dw_operand(kept + K.q, K.ldq, N), Operand{hs, D, 1}, V, D, dw_k(N), dW, GH_BF16, D,
+                           nullptr, nullptr, 0, nullptr, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
     return rc;
   if (dH && (rc = dh_gemm<__nv_bfloat16>(GH_BF16, Operand{kept + K.q, K.ldq, 0}, W, N, D, V, dH, nullptr, a,
                                          ws + L.dh2, status, slot, st)))
@@ -830,7 +853,7 @@ int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, co
       if ((rc = logits_gemm<T, gemm::EPI_LSM_GRAD>(Hc, W, rows, D, V, dtype, p, st))) return rc;
     }
     if (dW) {
-      lsm_clean_rows_kernel<T><<<4 * sms, 256, 0, st>>>(Hc, tgt + s0, arow + s0, rows, D / 8, hs);
+      lsm_clean_rows_kernel<T><<<4 * sms, 256, 0, st>>>(Hc, tgt + s0, arow + s0, rows, dw_pad(rows), D / 8, hs);
       count_launch(1);
       if ((rc = check_launch("lsm_clean_rows"))) return rc;
       void* out = dW;
@@ -844,8 +867,8 @@ int lsm_bwd_run(const void* H, const void* W, const int* tgt, const float* y, co
       } else if (!fp32_accum) {
         add_same = first ? nullptr : dW;
       }
-      if ((rc = run_gemm(dtype, Operand{d, L.ldd, 1}, Operand{hs, D, 1}, V, D, rows, out, out_dtype, D, add_f32,
-                         add_same, D, unscale, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
+      if ((rc = run_gemm(dtype, dw_operand(d, L.ldd, rows), Operand{hs, D, 1}, V, D, dw_k(rows), out, out_dtype, D,
+                         add_f32, add_same, D, unscale, 1, sms, st, status, PROF_GEMM_DW, kStreamA_KeepB)))
         return rc;
     }
     if (dH && (rc = dh_gemm<T>(dtype, Operand{d, L.ldd, 0}, W, rows, D, V, static_cast<T*>(dH) + s0 * D, unscale,

@@ -91,6 +91,7 @@ struct Params {
   // > 0 (256-column tiles): slice s writes at out + s * split_bytes instead, for
   // any number of slices; every slice holds at least one 64-wide k-step
   int64_t split_bytes;
+  int k_wrap;           // > 0: A's k-steps start over after this many
   int vec_ok;           // 16-byte aligned rows (vector stores allowed)
   const float* add_f32; // optional fp32 addend [M, ldadd]
   const void* add_same; // optional addend in the output type [M, ldadd]
@@ -514,13 +515,14 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           uint8_t* a = sA + stage * G::A_BYTES;
           uint8_t* b = sB + stage * G::B_BYTES;
           const int k0 = kb * BK;
+          const int ka = p.k_wrap && kb >= p.k_wrap ? k0 - p.k_wrap * BK : k0;
           if (PAIR == 1) {
             tc::mbar_arrive_expect_tx(&full[stage], G::A_BYTES + G::B_BYTES);
             if (A_MN) {
 #pragma unroll
-              for (int j = 0; j < BM / 64; ++j) tc::tma_load_2d_hint(a + j * (BK * 128), &tmA, &full[stage], ma + j * 64, k0, pol_a);
+              for (int j = 0; j < BM / 64; ++j) tc::tma_load_2d_hint(a + j * (BK * 128), &tmA, &full[stage], ma + j * 64, ka, pol_a);
             } else {
-              tc::tma_load_2d_hint(a, &tmA, &full[stage], k0, ma, pol_a);
+              tc::tma_load_2d_hint(a, &tmA, &full[stage], ka, ma, pol_a);
             }
             if (B_MN) {
 #pragma unroll
@@ -535,9 +537,9 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const uint32_t fb = tc::mapa_shared(tc::smem_u32(&full[stage]), 0);
             if (A_MN) {
 #pragma unroll
-              for (int j = 0; j < BM / 64; ++j) tc::tma_load_2d_pair_hint(a + j * (BK * 128), &tmA, fb, ma + j * 64, k0, pol_a);
+              for (int j = 0; j < BM / 64; ++j) tc::tma_load_2d_pair_hint(a + j * (BK * 128), &tmA, fb, ma + j * 64, ka, pol_a);
             } else {
-              tc::tma_load_2d_pair_hint(a, &tmA, fb, k0, ma, pol_a);
+              tc::tma_load_2d_pair_hint(a, &tmA, fb, ka, ma, pol_a);
             }
 #pragma unroll
             for (int h = 0; h < NSUB; ++h) {

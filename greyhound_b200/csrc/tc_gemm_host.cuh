@@ -19,6 +19,9 @@ struct Operand {
   const void* ptr;
   int64_t ld;
   int mn_major;  // 0: [rows, K] K contiguous; 1: [K, rows] rows contiguous
+  // > 0 (A): only this much of K is there; K = 2 * wrap rounded up to 64 takes it
+  // twice, each time with zeros up to the round number
+  int64_t wrap = 0;
 };
 
 // L2 policies of one GEMM: operand loads (0 none, 1 evict_first, 2 evict_last)
@@ -250,8 +253,9 @@ inline int pick_nsub(int64_t M, int64_t N, int pair, int units, bool fp32_epilog
 int make_operand_maps(CUtensorMap* ta, CUtensorMap* tb, int dtype, const Operand& A, const Operand& B, int64_t M,
                       int64_t N, int64_t K, int pair) {
   int rc;
-  if (A.mn_major) rc = make_map(ta, A.ptr, dtype, M, K, A.ld, BK);
-  else rc = make_map(ta, A.ptr, dtype, K, M, A.ld, BM);
+  const int64_t ka = A.wrap ? A.wrap : K;
+  if (A.mn_major) rc = make_map(ta, A.ptr, dtype, M, ka, A.ld, BK);
+  else rc = make_map(ta, A.ptr, dtype, ka, M, A.ld, BM);
   if (rc) return rc;
   if (B.mn_major) rc = make_map(tb, B.ptr, dtype, N, K, B.ld, BK);
   else rc = make_map(tb, B.ptr, dtype, K, N, B.ld, BN / pair);

@@ -101,6 +101,39 @@ def test_against_definition(N, D, V, dtype):
 
 @requires_gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("N,D,V", [(1, 512, 1000), (2, 64, 300), (63, 264, 513), (64, 128, 900), (65, 520, 1000), (128, 72, 4099)])
+def test_few_rows_round_the_weight_gradient_once(N, D, V, dtype, kept, monkeypatch):
+    """Up to 128 rows the second operand of dW's product comes in two parts, u^2 off
+    together (plus half of fp16's spacing, 2^-25). The target's term then carries
+    that alone, the others two roundings (stored or written, and the row's
+    factor), and the result its own u: beside the terms of `definition`
+    u |result| + 2 u sum |others| + 2^-14 sum |terms|, with 2^-14 above u^2 and the
+    fp32 steps before."""
+    if not kept:
+        monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    poison = torch.full((1 << 24,), float("nan"), device="cuda")  # what the buffers may find
+    del poison
+    H, W, t, g = make(N, D, V, dtype, N + D, scale=2.0)
+    h, w = H.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    (dw,) = torch.autograd.grad(chunked_linear_selective_log_softmax(h, w, t), w, g)
+    u, (_, _, rW, ey, _, _) = U[dtype], definition(H, W, t, g)
+    p = torch.softmax(H.double() @ W.double().T, 1)
+    on, at = t != -100, t.clamp(min=0)[:, None]
+    ga = torch.where(on, g.double().abs(), 0.0)[:, None]
+    others = (ga * p).scatter(1, at, 0.0)
+    terms = others.scatter(1, at, ga * (1 - p.gather(1, at)))
+    Ha = H.double().abs()
+    bound = u * rW.abs() + (2 * u * others + 2.0**-14 * terms + ey * ga * p).T @ Ha + 2.0**-62 * (ga * Ha).sum(0)
+    if dtype == torch.float16:
+        top = torch.nn.functional.pad(p, (0, -V % 128)).view(N, -1, 128).amax(2).repeat_interleave(128, 1)[:, :V]
+        e = 2.0**-25 * ga * top + 2.0**-37 * ga.amax()
+        bound += e.T @ Ha + 2.0**-24 * terms.sum(0)[:, None] + 2.0**-24
+    assert ((dw.double() - rW).abs() <= bound).all(), ((dw.double() - rW).abs() / bound).max()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("temperature", [0.3, 1.7])
 def test_temperature(dtype, temperature):
     check(*make(200, 128, 3001, dtype, 5, scale=1.5), temperature=temperature)
