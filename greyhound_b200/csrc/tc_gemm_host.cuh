@@ -69,9 +69,9 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
 }
 
 // 2-D map over a row-major matrix [outer, inner] with row pitch `ld`
-// elements, box {64, box_outer}, 128-byte swizzle, zero fill out of bounds.
-int make_map(CUtensorMap* map, const void* ptr, int dtype, int64_t inner, int64_t outer, int64_t ld,
-             int box_outer) {
+// elements, box {box_inner, box_outer}, zero fill out of bounds.
+int make_map(CUtensorMap* map, const void* ptr, int dtype, int64_t inner, int64_t outer, int64_t ld, int box_outer,
+             int box_inner = 64, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   // A host thread that has made no runtime call yet (autograd's backward
   // thread for device 0, for one) has no current context, and the driver
   // call below needs one: bind the current device's primary context.
@@ -87,10 +87,10 @@ int make_map(CUtensorMap* map, const void* ptr, int dtype, int64_t inner, int64_
   CUtensorMapDataType dt = dtype == GH_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
   cuuint64_t gstride[1] = {(cuuint64_t)(ld * elt)};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_outer};
+  cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(GH_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return GH_OK;
@@ -111,6 +111,18 @@ template <typename T, int A_MN, int B_MN, int EPI, typename OutT, int PAIR, int 
 int launch_gemm_t(const CUtensorMap& ta, const CUtensorMap& tb, gemm::Params& p, int max_ctas, cudaStream_t st) {
   auto kern = gemm::tc_gemm_kernel<T, A_MN, B_MN, EPI, OutT, PAIR, NSUB>;
   constexpr int SMEM = gemm::Geo<PAIR, NSUB>::SMEM;
+  CUtensorMap to{};
+  p.bulk_out = 0;
+  if constexpr (gemm::bulk_output<EPI, OutT, NSUB>()) {
+    // EPI_STORE: one output without an addend, its rows 16-byte aligned
+    if (EPI != gemm::EPI_STORE ||
+        (p.vec_ok && p.out && p.ksplit <= 1 && !p.split_bytes && p.npeer <= 0 && !p.add_f32 && !p.add_same)) {
+      const int rc = make_map(&to, p.out, gemm::AbType<OutT>::v ? GH_BF16 : GH_F16, p.N, p.M, p.ldo, 32, 32,
+                              CU_TENSOR_MAP_SWIZZLE_64B);
+      if (rc) return rc;
+      p.bulk_out = 1;
+    }
+  }
   static int max_units[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -154,7 +166,7 @@ int launch_gemm_t(const CUtensorMap& ta, const CUtensorMap& tb, gemm::Params& p,
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, to, p);
   if (e != cudaSuccess) return set_error(GH_ECUDA, "tc_gemm launch: %s", cudaGetErrorString(e));
   count_launch(1);
   return check_launch("tc_gemm");
