@@ -8,6 +8,7 @@ linear cross-entropy takes the cross-entropy.
 
 from __future__ import annotations
 
+import functools
 import math
 import os
 
@@ -63,8 +64,21 @@ def _operand(t: Tensor) -> Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+# Sizes decide this and the workspaces' bytes; worked out once per shape (the
+# backward runs on autograd's thread, where every line costs twice as much).
+@functools.lru_cache(maxsize=1024)
 def _chunk(N: int, D: int, V: int) -> int:
     return chunk_size_for(N, D, V, 2) if N > 0 else 1
+
+
+@functools.lru_cache(maxsize=1024)
+def _forward_bytes(N: int, V: int, chunk: int, keep: bool) -> int:
+    return _lib.load().gh_lsm_fwd_workspace_bytes(N, V, chunk, int(keep))
+
+
+@functools.lru_cache(maxsize=1024)
+def _backward_bytes(N: int, D: int, V: int, chunk: int, code: int, kept: bool, fp32: bool) -> int:
+    return _lib.load().gh_lsm_bwd_workspace_bytes(N, D, V, chunk, code, int(kept), int(fp32))
 
 
 def kept_bytes(N: int, V: int, dtype: torch.dtype) -> int:
@@ -109,7 +123,7 @@ def linear_logprobs(
             return out, state, kept
         x, w, idx = _operand(inputs), _operand(weight), index.contiguous()
         chunk = _chunk(N, D, V)
-        ws = _lib.workspace(lib.gh_lsm_fwd_workspace_bytes(N, V, chunk, int(keep)), dev)
+        ws = _lib.workspace(_forward_bytes(N, V, chunk, keep), dev)
         st = lib.gh_lsm_fwd(
             x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), N, D, V,
             _lib.dtype_code(x.dtype), int(ignore_index), 1.0 / float(temperature), chunk, out.data_ptr(),
@@ -123,8 +137,10 @@ def linear_logprobs(
 
 def _check_grad(grad: Tensor, inputs: Tensor) -> Tensor:
     if grad.shape != (inputs.shape[0],) or grad.device != inputs.device:
-        raise ValueError(f"expected grad shape {(inputs.shape[0],)} on {inputs.device}, got {tuple(grad.shape)} on {grad.device}")
-    return grad.to(torch.float32).contiguous()
+        raise ValueError(
+            f"expected grad shape {(inputs.shape[0],)} on {inputs.device}, got {tuple(grad.shape)} on {grad.device}"
+        )
+    return grad if grad.dtype is torch.float32 and grad.is_contiguous() else grad.to(torch.float32).contiguous()
 
 
 def linear_logprobs_backward_kept(
@@ -145,14 +161,14 @@ def linear_logprobs_backward_kept(
     with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax backward")
         x, w, g = _operand(inputs), _operand(weight), _check_grad(grad, inputs)
-        gi = torch.empty((N, D), dtype=inputs.dtype, device=dev) if want_input else None
-        gw = torch.empty((V, D), dtype=weight.dtype, device=dev) if want_weight else None
+        gi = torch.empty_like(x) if want_input else None
+        gw = torch.empty_like(w) if want_weight else None
         if N == 0:
             return gi, gw.zero_() if gw is not None else None
-        chunk, code, fp32 = _chunk(N, D, V), _lib.dtype_code(x.dtype), int(fp32_grad_weight_accum)
-        ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, code, 1, fp32), dev)
+        chunk, code, fp32 = _chunk(N, D, V), _lib.dtype_code(x.dtype), bool(fp32_grad_weight_accum)
+        ws = _lib.workspace(_backward_bytes(N, D, V, chunk, code, True, fp32), dev)
         st = lib.gh_lsm_bwd_kept(
-            x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, code, 1.0 / float(temperature), chunk, fp32,
+            x.data_ptr(), w.data_ptr(), g.data_ptr(), N, D, V, code, 1.0 / float(temperature), chunk, int(fp32),
             kept.data_ptr(), kept.numel(), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(),
             _lib.stream_handle(dev),
         )
@@ -184,18 +200,16 @@ def linear_logprobs_backward(
     with _lib.on_device(dev):
         _lib.raise_pending(dev, "linear_selective_log_softmax backward")
         x, w, idx, g = _operand(inputs), _operand(weight), index.contiguous(), _check_grad(grad, inputs)
-        gi = torch.empty((N, D), dtype=inputs.dtype, device=dev) if want_input else None
-        gw = torch.empty((V, D), dtype=weight.dtype, device=dev) if want_weight else None
+        gi = torch.empty_like(x) if want_input else None
+        gw = torch.empty_like(w) if want_weight else None
         if N == 0:
             return gi, gw.zero_() if gw is not None else None
-        chunk = _chunk(N, D, V)
-        ws = _lib.workspace(lib.gh_lsm_bwd_workspace_bytes(N, D, V, chunk, _lib.dtype_code(x.dtype), 0,
-                                                            int(fp32_grad_weight_accum)), dev)
+        chunk, code, fp32 = _chunk(N, D, V), _lib.dtype_code(x.dtype), bool(fp32_grad_weight_accum)
+        ws = _lib.workspace(_backward_bytes(N, D, V, chunk, code, False, fp32), dev)
         st = lib.gh_lsm_bwd(
             x.data_ptr(), w.data_ptr(), idx.data_ptr(), _lib.dtype_code(idx.dtype), state.data_ptr(),
-            g.data_ptr(), N, D, V, _lib.dtype_code(x.dtype), int(ignore_index),
-            1.0 / float(temperature), chunk, int(fp32_grad_weight_accum), _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(),
-            ws.numel(), _lib.stream_handle(dev),
+            g.data_ptr(), N, D, V, code, int(ignore_index), 1.0 / float(temperature), chunk, int(fp32),
+            _lib.ptr(gi), _lib.ptr(gw), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
         )
         _lib.check(st, "linear_selective_log_softmax backward")
         _lib.raise_on_status(ws, "linear_selective_log_softmax backward")

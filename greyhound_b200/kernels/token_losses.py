@@ -7,6 +7,7 @@ offsets ``cu_seqlens``; a boolean mask may leave positions out.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -89,9 +90,15 @@ def _seqs(logprobs: Tensor, cu_seqlens: Tensor | None) -> int:
     return cu_seqlens.numel() - 1 if cu_seqlens is not None else logprobs.shape[0] if logprobs.ndim == 2 else 1
 
 
+@functools.lru_cache(maxsize=1024)  # sizes alone decide it
 def _policy_workspace(tokens: int, seqs: int, reduction: str) -> int:
     """Floats of the policy loss's workspace, rounded to 16 bytes."""
     return (int(_lib.load().gh_policy_loss_workspace_bytes(tokens, seqs, REDUCTIONS[reduction])) + 15) // 16 * 4
+
+
+@functools.lru_cache(maxsize=1024)
+def _preference_workspace(tokens: int, seqs: int) -> int:
+    return _lib.load().gh_preference_loss_workspace_bytes(tokens, seqs)
 
 
 def policy_state_size(logprobs: Tensor, cu_seqlens: Tensor | None, reduction: str, want_grad: bool) -> int:
@@ -254,7 +261,7 @@ def preference_loss_forward(
         loss = torch.empty((), dtype=torch.float32, device=dev)
         state = torch.empty(2, lay.seqs, dtype=torch.float32, device=dev)
         at = state.data_ptr()
-        ws = _lib.workspace(lib.gh_preference_loss_workspace_bytes(lay.tokens, lay.seqs), dev)
+        ws = _lib.workspace(_preference_workspace(lay.tokens, lay.seqs), dev)
         st = lib.gh_preference_loss_fwd(
             lp.data_ptr(), _lib.dtype_code(lp.dtype), _lib.ptr(ref), other, _lib.ptr(m), lay.tokens,
             _lib.ptr(lay.cu), lay.cu_code, lay.seqs, float(beta), float(margin), float(label_smoothing),
