@@ -321,8 +321,19 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def untraced() -> bool:
+    """Whether calls are run only, and not recorded: what goes past the dispatcher would be
+    missing from the record of ``torch.compile``, of a dispatch mode (``make_fx``, fake
+    tensors, any ``TorchDispatchMode``) or of ``torch.jit.trace``."""
+    return (
+        not torch.compiler.is_compiling()  # first: all that torch.compile itself gets to see
+        and torch._C._len_torch_dispatch_stack() == 0
+        and torch._C._get_tracing_state() is None
+    )
+
+
 def eager(t: torch.Tensor) -> bool:
     """Whether ``t`` is a plain tensor outside of any tracing: the autograd
     Functions then call a kernel's wrapper itself, as its custom op would
     (the op's own Python layers cost some 80 us a call)."""
-    return type(t) in (torch.Tensor, torch.nn.Parameter) and not torch.compiler.is_compiling()
+    return untraced() and type(t) in (torch.Tensor, torch.nn.Parameter)
