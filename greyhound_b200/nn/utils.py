@@ -13,7 +13,7 @@ from collections.abc import Iterable, Sequence
 import torch
 from torch import Tensor
 
-from greyhound_b200.kernels.grad_norm import clip_tensors
+from greyhound_b200.ops.grad_norm import clip
 
 __all__ = ["clip_by_global_norm", "clip_grad_norm_", "global_norm"]
 
@@ -34,7 +34,7 @@ def global_norm(tensors: Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
     ts = list(tensors)
     if not ts:
         return torch.zeros((), dtype=torch.float32, device=_device(ts))
-    return clip_tensors(ts, None, 0.0, float(norm_type), _device(ts))
+    return clip(ts, None, 0.0, float(norm_type))
 
 
 def clip_by_global_norm(
@@ -62,7 +62,7 @@ def clip_by_global_norm(
         if outs:
             raise ValueError(f"expected 0 outputs, got {len(outs)}")
         return [], torch.zeros((), dtype=torch.float32, device=_device(ts))
-    return outs, clip_tensors(ts, outs, float(max_norm), float(norm_type), _device(ts))
+    return outs, clip(ts, outs, float(max_norm), float(norm_type))
 
 
 def clip_grad_norm_(
@@ -90,7 +90,7 @@ def clip_grad_norm_(
     if not float(max_norm) >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if error_if_nonfinite:
-        norm = clip_tensors(grads, None, 0.0, float(norm_type), _device(grads))
+        norm = clip(grads, None, 0.0, float(norm_type))
         if not math.isfinite(norm.item()):
             raise RuntimeError(f"the norm of the gradients is {norm.item()}; they were not clipped")
-    return clip_tensors(grads, grads, float(max_norm), float(norm_type), _device(grads))
+    return clip(grads, grads, float(max_norm), float(norm_type))

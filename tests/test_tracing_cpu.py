@@ -1,6 +1,6 @@
-"""What a trace records of the log-probabilities and the token losses: their custom ops,
-forward and backward. The kernels' wrappers are replaced by ones that write 7.0 past
-the dispatcher, as the C entries do."""
+"""What a trace records of the log-probabilities, the token losses and the clipping: their
+custom ops, forward and backward. The kernels' wrappers are replaced by ones that write
+past the dispatcher, as the C entries do."""
 
 import ctypes
 
@@ -9,9 +9,10 @@ import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
+from greyhound_b200.nn import utils
 from greyhound_b200.nn.functional import chunked_linear_selective_log_softmax, clipped_policy_loss, preference_loss
 from greyhound_b200.ops import chunked_linear_selective_log_softmax as lsm
-from greyhound_b200.ops import token_losses
+from greyhound_b200.ops import grad_norm, token_losses
 
 
 def written(*shape, dtype=torch.float32):
@@ -110,3 +111,88 @@ def test_outside_of_tracing_no_op_is_called(kernels, step, shape, ops, monkeypat
         module = token_losses if "loss" in name else lsm
         monkeypatch.setattr(module, name, None)
     assert (step(torch.ones(*shape, requires_grad=True))[0] == 7.0).all()
+
+
+@pytest.fixture
+def clipping(monkeypatch):
+    def tensors(ts, outs, max_norm, kind, device):
+        for t, o in zip(ts, outs or ()):
+            half = t.detach() * 0.5
+            ctypes.memmove(o.data_ptr(), half.data_ptr(), o.numel() * 4)
+            torch.autograd.graph.increment_version(o)
+        return written()
+
+    monkeypatch.setattr(grad_norm, "clip_tensors", tensors)
+
+
+def norm_alone(a, b):
+    return (utils.global_norm([a, b]),)
+
+
+def clipped_copies(a, b):
+    (x, y), n = utils.clip_by_global_norm([a, b], 1.0)
+    return x + 1.0, y + 1.0, n
+
+
+def clipped_in_place(a, b):
+    ts = [a + 1.0, b + 1.0]
+    _, n = utils.clip_by_global_norm(ts, 1.0, out=ts)
+    return ts[0] * 3.0, ts[1] * 3.0, n
+
+
+def one_in_place(a, b):
+    a, b, c = a + 1.0, b + 1.0, torch.empty_like(b)
+    _, n = utils.clip_by_global_norm([a, b], 1.0, out=[a, c])
+    return a * 3.0, b * 3.0, c * 3.0, n
+
+
+def parameters(a, b):
+    p, q = torch.nn.Parameter(a + 1.0), torch.nn.Parameter(b + 1.0)
+    p.grad, q.grad = a + 2.0, b + 3.0
+    n = utils.clip_grad_norm_([p, q], 1.0)
+    return p.grad * 3.0, q.grad * 3.0, n
+
+
+CLIPS = [
+    (norm_alone, {"global_norm"}),
+    (clipped_copies, {"clip_by_global_norm_out"}),
+    (clipped_in_place, {"clip_by_global_norm_"}),
+    (one_in_place, {"clip_by_global_norm_out"}),
+    (parameters, {"clip_by_global_norm_"}),
+]
+
+
+@pytest.mark.parametrize("mode", ["real", "fake"])
+@pytest.mark.parametrize("step,ops", CLIPS)
+def test_make_fx_records_the_clipping(clipping, step, ops, mode):
+    a, b = torch.randn(3), torch.randn(2, 5)
+    graph = make_fx(step, tracing_mode=mode)(a, b)
+    assert {n.target._opname for n in graph.graph.nodes if getattr(n.target, "namespace", "") == "greyhound"} == ops
+    for _ in range(2):
+        for got, want in zip(graph(a, b), step(a, b)):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("step,ops", CLIPS)
+def test_dispatch_modes_see_the_clipping(clipping, step, ops):
+    with Recorder() as seen:
+        step(torch.randn(3), torch.randn(2, 5))
+    assert seen.ops == ops
+
+
+@pytest.mark.parametrize("step", [s for s, _ in CLIPS if s is not parameters])
+def test_jit_traces_hold_the_clipping(clipping, step):
+    a, b = torch.randn(3), torch.randn(2, 5)
+    graph = torch.jit.trace(step, (a, b), check_trace=False)
+    a, b = torch.randn(3), torch.randn(2, 5)
+    for got, want in zip(graph(a, b), step(a, b)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("step", [s for s, _ in CLIPS if s is not parameters])
+def test_compiled_clipping(clipping, step):
+    a, b = torch.randn(3), torch.randn(2, 5)
+    torch._dynamo.reset()
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    for got, want in zip(compiled(a, b), step(a, b)):
+        assert torch.equal(got, want)
