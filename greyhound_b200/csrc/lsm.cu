@@ -484,15 +484,15 @@ Operand dw_operand(const void* d, int64_t ldd, int64_t rows) { return Operand{d,
 // pairs of SMs, 157 us), while K is long: the slices' fp32 sums are written to
 // memory and joined. Modelled in us: 0.38 a k-step of a 256 x 256 pair tile
 // (measured at full load), 12 k-steps a tile for its ends, the slices' traffic
-// at 5 TB/s. 0: run_gemm's own choice (two 16-bit halves at most) is as good.
+// at 5 TB/s. 0: the product is taken whole. (run_gemm's own split is of no use
+// here: its two partial sums are rounded to 16 bits before they are added.)
 int dh_slices(int64_t rows, int64_t D, int64_t V) {
   const int pair = pick_pair(rows);
   const int64_t units = num_sms_dev() / pair;
   const int64_t tiles = (rows + BM * pair - 1) / (BM * pair) * ((D + BN - 1) / BN);
   const int64_t nkb = (V + BK - 1) / BK;
   auto waves = [&](int64_t t) { return (double)((t + units - 1) / units); };
-  double best = 0.9 * (nkb >= 32 && pair == 2 && D > BN ? waves(tiles) * ((double)nkb / 2 + 12) * 0.72 + 4.0
-                                                       : waves(tiles) * ((double)nkb + 12) * 0.38);
+  double best = 0.9 * waves(tiles) * ((double)nkb + 12) * 0.38;
   int slices = 0;
   for (int s = 2; s <= 64 && nkb / s >= 8; ++s) {
     const int64_t per = (nkb + s - 1) / s, n = (nkb + per - 1) / per;  // no empty slice
@@ -506,12 +506,8 @@ int dh_slices(int64_t rows, int64_t D, int64_t V) {
   return slices;
 }
 
-// Bytes of the second product's scratch: the slices in fp32, or run_gemm's
-// second 16-bit half.
-size_t dh_scratch(int64_t rows, int64_t D, int64_t V) {
-  const int s = dh_slices(rows, D, V);
-  return (size_t)rows * D * (s ? (size_t)s * 4 : 2);
-}
+// Bytes of the product's scratch: the slices in fp32.
+size_t dh_scratch(int64_t rows, int64_t D, int64_t V) { return (size_t)rows * D * dh_slices(rows, D, V) * 4; }
 
 // dH[rows, D] = row[r] * scale * (A[rows, V] W[V, D]). Where slices are joined,
 // the join hands the status on to `slot`.
@@ -521,9 +517,9 @@ int dh_gemm(int dtype, const Operand& A, const void* W, int64_t rows, int64_t D,
   const int slices = dh_slices(rows, D, V);
   const int sms = num_sms_dev();
   const Operand B{W, D, 1};
-  if (!slices)  // fp16: two 16-bit halves would round twice, near zero by a step each
+  if (!slices)
     return run_gemm(dtype, A, B, rows, D, V, out, dtype, D, nullptr, nullptr, 0, scale, 1, sms, st, status,
-                    PROF_GEMM_DH, Hints{}, dtype == GH_F16 ? nullptr : scratch, row);
+                    PROF_GEMM_DH, Hints{}, nullptr, row);
   const int pair = pick_pair(rows);
   CUtensorMap ta, tb;
   int rc = make_operand_maps(&ta, &tb, dtype, A, B, rows, D, V, pair);

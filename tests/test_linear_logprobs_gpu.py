@@ -454,3 +454,46 @@ def test_result_may_be_changed_in_place(monkeypatch, kept):
     y = chunked_linear_selective_log_softmax(h, W, t)
     y.mul_(2.0)
     assert torch.allclose(torch.autograd.grad(y, h, g / 2)[0].float(), dh.float(), rtol=2.0**-7, atol=1e-6)
+
+
+@requires_gpu
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("N,D,V", [(3000, 1024, 2048), (1100, 2048, 4096)])
+def test_partial_sums_of_the_input_gradient_keep_32_bits(monkeypatch, N, D, V, kept):
+    """The two halves of the vocabulary cancel: W is 1 + n in one and -1 + n in the other, p is
+    even over both, so that dH = g (W_t - sum p W), with W_t = 0, is small beside its halves of g / 2.
+    Some columns of W are random, so that the logits spread by 1/2 and e^x over many 16-bit steps.
+
+    A sum held in 32 bits leaves: the result's rounding u |dH|; the row factor, which takes the
+    target's rounding (u at most) off the row's other entries together, u |dH|; the
+    log-probability's error ey |dH| likewise; each e^x's own rounding, of at most u and independent:
+    by Hoeffding's inequality their sum stays below
+    sqrt(2 ln(2 10^13)) u (sum (p W)^2)^(1/2) = 7.9 u (...) for all of 10^7 values but in one draw of
+    10^6; and the tensor core's truncation, 2^-23 of the running sum at each of the V / 16 steps.
+    16-bit halves would add up to 2^-8 g together."""
+    if not kept:
+        monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    u = U[torch.bfloat16]
+    gen = torch.Generator(device="cuda").manual_seed(35)
+    H = torch.zeros(N, D, device="cuda")
+    H[:, :64] = torch.randn(N, 64, device="cuda", generator=gen) / 16
+    H = H.bfloat16()
+    W = torch.randn(V, D, device="cuda", generator=gen) * 0.02
+    W[: V // 2] += 1.0
+    W[V // 2 :] -= 1.0
+    W[:, :64] = torch.randn(V, 64, device="cuda", generator=gen)
+    W = W.bfloat16()
+    t = torch.randint(0, V, (N,), device="cuda", generator=gen) // 64 * 64
+    W[::64] = 0.0
+    g = 1.0 + torch.rand(N, device="cuda", generator=gen)
+    h = H.clone().requires_grad_(True)
+    (dh,) = torch.autograd.grad(chunked_linear_selective_log_softmax(h, W, t), h, g)
+    Wd = W.double()
+    p = torch.softmax(H.double() @ Wd.T, 1)
+    ga = g.double()[:, None]
+    want = -ga * (p @ Wd)  # W_t = 0
+    S = (H.double().abs() @ Wd.abs().T).amax()
+    ey = 2 * (D / 16 + 4) * 2.0**-23 * S + 2.0**-20
+    bound = (2 * u + ey) * want.abs() + ga * (7.9 * u * (p**2 @ Wd**2).sqrt() + V / 16 * 2.0**-23 * (p @ Wd.abs()))
+    err = (dh.double() - want).abs()
+    assert (err <= bound).all(), (err / bound).max()
