@@ -752,8 +752,8 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
     if (!kept) {
       int few = 0;
       if (N <= kFewRows) {
-        if (N == 1) rc = few_rows<T, 1>(Hc, W, tgt, rows, D, V, sc2, stats, &few, xt, st);
-        else rc = few_rows<T, kFewRows>(Hc, W, tgt, rows, D, V, sc2, stats, &few, xt, st);
+        if (N == 1) rc = few_rows<T, 1>(Hc, W, tgt + s0, rows, D, V, sc2, stats, &few, xt, st);
+        else rc = few_rows<T, kFewRows>(Hc, W, tgt + s0, rows, D, V, sc2, stats, &few, xt, st);
         if (rc) return rc;
       }
       if (few) parts = few;

@@ -497,3 +497,16 @@ def test_partial_sums_of_the_input_gradient_keep_32_bits(monkeypatch, N, D, V, k
     bound = (2 * u + ey) * want.abs() + ga * (7.9 * u * (p**2 @ Wd**2).sqrt() + V / 16 * 2.0**-23 * (p @ Wd.abs()))
     err = (dh.double() - want).abs()
     assert (err <= bound).all(), (err / bound).max()
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("left_out", [None, 0, 1])
+def test_scoring_two_rows_in_two_chunks(monkeypatch, dtype, left_out):
+    """Each row with its own target, whatever the rows of a chunk."""
+    H, W, t, g = make(2, 264, 4099, dtype, 31, scale=3.0, left_out=0.0)
+    if left_out is not None:
+        t[left_out] = -100
+    monkeypatch.setattr(K, "_chunk", lambda N, D, V: 1)
+    y = chunked_linear_selective_log_softmax(H, W, t)
+    ry, _, _, ey, _, _ = definition(H, W, t, g)
+    assert ((y.double() - ry).abs() <= ey).all(), (y, ry)
