@@ -766,6 +766,12 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
     count_launch(1);
     if ((rc = check_launch("lsm_combine"))) return rc;
   }
+  if (own_state && state) {  // both were asked for: the kept buffer's copy is the caller's, too
+    const cudaError_t e1 = cudaMemcpyAsync(state, lse2, sizeof(float) * N, cudaMemcpyDeviceToDevice, st);
+    const cudaError_t e2 = cudaMemcpyAsync(state + N, y2, sizeof(float) * N, cudaMemcpyDeviceToDevice, st);
+    if (e1 != cudaSuccess || e2 != cudaSuccess)
+      return set_error(GH_ECUDA, "copy of the state: %s", cudaGetErrorString(e1 != cudaSuccess ? e1 : e2));
+  }
   return GH_OK;
 }
 

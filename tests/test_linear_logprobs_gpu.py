@@ -25,6 +25,7 @@ import pytest
 import torch
 from torch.library import opcheck
 
+from greyhound_b200 import _lib
 from greyhound_b200.kernels import linear_logprobs as K
 from greyhound_b200.nn.functional import chunked_linear_selective_log_softmax
 from greyhound_b200.ops.chunked_linear_selective_log_softmax import (
@@ -510,3 +511,31 @@ def test_scoring_two_rows_in_two_chunks(monkeypatch, dtype, left_out):
     y = chunked_linear_selective_log_softmax(H, W, t)
     ry, _, _, ey, _, _ = definition(H, W, t, g)
     assert ((y.double() - ry).abs() <= ey).all(), (y, ry)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_c_entry_writes_state_beside_the_kept_buffer(dtype):
+    """`state` and `kept` are independent: asking for both gives what each alone does."""
+    H, W, t, _ = make(300, 128, 1111, dtype, 32)
+    lib = _lib.load()
+    N, D, V, code = 300, 128, 1111, _lib.dtype_code(dtype)
+
+    def forward(state, kept):
+        out = torch.full((N,), float("nan"), device="cuda")
+        ws = _lib.workspace(lib.gh_lsm_fwd_workspace_bytes(N, V, N, int(kept is not None)), H.device)
+        st = lib.gh_lsm_fwd(
+            H.data_ptr(), W.data_ptr(), t.data_ptr(), _lib.GH_I64, N, D, V, code, -100, 1.0, N, out.data_ptr(),
+            _lib.ptr(state), _lib.ptr(kept), 0 if kept is None else kept.numel(), ws.data_ptr(), ws.numel(),
+            _lib.stream_handle(H.device),
+        )
+        _lib.check(st, "forward")
+        return out
+
+    alone, both = (torch.full((2, N), float("nan"), device="cuda") for _ in range(2))
+    kept = torch.zeros(K.kept_bytes(N, V, dtype), dtype=torch.uint8, device="cuda")
+    only = torch.zeros_like(kept)
+    y = forward(alone, None)
+    assert torch.equal(forward(both, kept), y) and torch.equal(forward(None, only), y)
+    assert torch.equal(alone, both) and torch.isfinite(both).all()
+    assert torch.equal(kept, only)
