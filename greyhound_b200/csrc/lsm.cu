@@ -759,7 +759,9 @@ int lsm_fwd_run(const void* H, const void* W, int64_t N, int64_t D, int64_t V, i
       if (few) parts = few;
       else if ((rc = logits_gemm<T, gemm::EPI_LSM>(Hc, W, rows, D, V, dtype, p, st))) return rc;
     }
-    if (rows <= 4 * (int64_t)num_sms_dev())
+    // by all rows, not the chunk's: a short last chunk adds its tiles in the order
+    // in which a pass that takes them all at once does
+    if (N <= 4 * (int64_t)num_sms_dev())
       lsm_combine_kernel<1><<<(unsigned)rows, 256, 0, st>>>(stats, parts, rows, V, sc2, xt, tgt + s0, o);
     else
       lsm_combine_kernel<8><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(stats, parts, rows, V, sc2, xt, tgt + s0, o);

@@ -832,7 +832,8 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           // exponent has no such window, shifts every group. Without the
           // store the sums are formed the same way, so that a scoring pass and
           // a training pass over the same rows agree in every bit (the ratio of
-          // their probabilities is exactly 1).
+          // their probabilities is exactly 1), unless there are only one or two,
+          // which a scoring pass gives to a kernel without tiles.
           const int t_rel = (row_ok ? p.tgt[row] : -1) - col_g;
           float cmax = kNegInf;
           if (col_g + NV <= p.N) {

@@ -539,3 +539,18 @@ def test_c_entry_writes_state_beside_the_kept_buffer(dtype):
     assert torch.equal(forward(both, kept), y) and torch.equal(forward(None, only), y)
     assert torch.equal(alone, both) and torch.isfinite(both).all()
     assert torch.equal(kept, only)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rest", [100, 300])
+def test_chunked_scoring_agrees_with_training_in_every_bit(monkeypatch, dtype, rest):
+    """A long chunk and a short last one against the kept forward's single chunk, over
+    125 vocabulary tiles: their statistics are added in one order whatever the chunks."""
+    H, W, t, _ = make(700 + rest, 192, 32_000, dtype, 33, scale=2.0)
+    h = H.clone().requires_grad_(True)
+    trained = chunked_linear_selective_log_softmax(h, W, t).detach()
+    monkeypatch.setattr(K, "_chunk", lambda N, D, V: 700)
+    assert torch.equal(chunked_linear_selective_log_softmax(H, W, t), trained)
+    monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    assert torch.equal(chunked_linear_selective_log_softmax(h, W, t).detach(), trained)
