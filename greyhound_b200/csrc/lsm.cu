@@ -26,7 +26,9 @@
 //              workspace whatever N.
 // Bound by the tensor pipe for many rows and by reading W once for few.
 #include <algorithm>
+#include <cfloat>
 #include <initializer_list>
+#include <type_traits>
 
 #include "row_ops.cuh"
 #include "tc_gemm_host.cuh"
@@ -275,7 +277,7 @@ lsm_combine_kernel(const float2* __restrict__ stats, int num_n, int64_t rows, in
         // its row. Its 16-bit rounding would reach dW on top of the one of a * H,
         // so the row factor takes it out: alpha0 * (stored target) is exact to
         // fp32, and the row's other entries, each rounded already, move by at
-        // most 2^-9.
+        // most 2^-8.
         const double tau = expm1(y) * (odd ? 1.0 : exp2(lse2));
         const __nv_bfloat16 c = __float2bfloat16_rn((float)tau);
         const double cd = (double)__bfloat162float(c);
@@ -294,12 +296,16 @@ lsm_combine_kernel(const float2* __restrict__ stats, int num_n, int64_t rows, in
   }
 }
 
-// Eight elements of the dW GEMM's second operand, in 16 bits. With lo > 0, what
-// the rounding took off follows lo vectors further on.
+// Eight elements of the dW GEMM's second operand, in 16 bits; finite ones stay
+// within +-most. With lo > 0, what the rounding took off follows lo vectors
+// further on.
 template <typename T>
-__device__ __forceinline__ void put_operand(T* hs, int64_t i, int64_t lo, const float (&f)[8]) {
+__device__ __forceinline__ void put_operand(T* hs, int64_t i, int64_t lo, const float (&f)[8], float most) {
+  float c[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) c[k] = fabsf(f[k]) <= FLT_MAX ? fminf(fmaxf(f[k], -most), most) : f[k];
   Vec16<T> v;
-  v.from_float(f);
+  v.from_float(c);
   st16(reinterpret_cast<uint4*>(hs) + i, v.raw);
   if (!lo) return;
   float r[8], rest[8];
@@ -334,7 +340,7 @@ lsm_rows_kernel(const __nv_bfloat16* __restrict__ H, const float* __restrict__ g
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] *= a;
     }
-    put_operand(hs, i, lo, f);
+    put_operand(hs, i, lo, f, FLT_MAX);
   }
 }
 
@@ -379,7 +385,9 @@ lsm_factor_kernel(const float* __restrict__ g, const float* __restrict__ y, cons
   const float f = on ? g[r] * inv_t * (scale ? scale[0] : 1.f) : 0.f;
   const float tv = on ? -f * expm1f(y[r]) : 0.f;
   const float c = Elt<T>::to_f(Elt<T>::from_f(tv));
-  const bool fit = c != 0.f && fabsf(c) <= 3.4e38f && fabsf(tv) >= 1e-30f;  // neither 0, inf nor NaN
+  // neither inf nor NaN, nor below the type's normal numbers, whose rounding is no small share of them
+  constexpr float least = std::is_same<T, __half>::value ? 0x1p-14f : 1e-30f;
+  const bool fit = fabsf(c) >= least && fabsf(c) <= 3.4e38f;
   rfac[r] = fit ? f * (c / tv) : f;
   tval[r] = fit ? c : tv;
   arow[r] = !on ? 0.f : fit ? tv / c : 1.f;
@@ -427,6 +435,9 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 lsm_clean_rows_kernel(const T* __restrict__ H, const int* __restrict__ tgt, const float* __restrict__ arow,
                       int64_t rows, int64_t pad, int64_t vpr, T* __restrict__ out) {
+  // arow is within a rounding of 1: the type's largest values may leave it, and
+  // inf times an entry of d that is 0 would be NaN
+  constexpr float most = std::is_same<T, __half>::value ? 65504.f : 3.3895314e38f;
   const int64_t n = (pad ? pad : rows) * vpr, lo = pad * vpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / vpr;
@@ -439,7 +450,7 @@ lsm_clean_rows_kernel(const T* __restrict__ H, const int* __restrict__ tgt, cons
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] *= a;
     }
-    put_operand(out, i, lo, f);
+    put_operand(out, i, lo, f, most);
   }
 }
 

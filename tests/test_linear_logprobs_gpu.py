@@ -554,3 +554,20 @@ def test_chunked_scoring_agrees_with_training_in_every_bit(monkeypatch, dtype, r
     assert torch.equal(chunked_linear_selective_log_softmax(H, W, t), trained)
     monkeypatch.setattr(K, "_KEEP_BYTES", 0)
     assert torch.equal(chunked_linear_selective_log_softmax(h, W, t).detach(), trained)
+
+
+@requires_gpu
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("N", [100, 300])
+def test_largest_fp16_hidden_value_with_a_small_gradient(monkeypatch, N, kept):
+    """65504 in scored rows whose gradients are 2^-20 to 2^-31 of the largest: the target's entry
+    is a subnormal number there, and the row's factor times 65504 must not leave fp16."""
+    if not kept:
+        monkeypatch.setattr(K, "_KEEP_BYTES", 0)
+    H, W, t, g = make(N, 64, 500, torch.float16, 34, left_out=0.0)
+    W[:, 3] *= 2.0**-14
+    H[::2, 3] = 65504.0
+    H[1::4, 3] = -65504.0
+    g[1:] = torch.sign(g[1:]) * 2.0 ** -torch.linspace(20, 31, N - 1, device="cuda")
+    g[0], H[0, 3] = 1.0, 0.5
+    check(H, W, t, g)
