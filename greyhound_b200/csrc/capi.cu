@@ -35,18 +35,16 @@ void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 // status into this device's slot (nothing crosses the bus when the status is
 // zero). The host reads and clears a slot with gh_take_device_errors() without
 // synchronising, so a problem recorded by call k is seen at call k + 1 or
-// later, once the GPU has run call k.
+// later, once the GPU has run call k. Kernels OR their bits in atomically
+// (report_bits); a read on the host in the middle of that may see a bit twice,
+// never lose one.
 namespace {
 constexpr int kMaxDevices = 64;
 std::once_flag g_slots_once;
 int* g_slots = nullptr;
 
 __global__ void publish_status_kernel(const int* __restrict__ status, int* slot) {
-  const int v = *reinterpret_cast<const volatile int*>(status);
-  if (v) {
-    volatile int* h = slot;
-    *h = *h | v;
-  }
+  report_bits(slot, *reinterpret_cast<const volatile int*>(status));
 }
 }  // namespace
 

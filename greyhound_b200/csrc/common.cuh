@@ -30,6 +30,12 @@ int publish_status(const int* status, cudaStream_t st);
 // Device address of the current device's sticky error slot, for a kernel that
 // reports a problem there itself.
 int device_error_slot(int** slot);
+// OR bits into that slot. Kernels of several streams, and many threads of one,
+// report at the same time: an atomic, so that none writes away what another has
+// just reported.
+__device__ __forceinline__ void report_bits(int* slot, int bits) {
+  if (bits) atomicOr(slot, bits);
+}
 
 // Kernel classes for the optional event timing (gh_profile_enable / _read).
 enum ProfClass {

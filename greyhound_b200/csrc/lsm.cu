@@ -65,13 +65,7 @@ lsm_targets_kernel(const I* __restrict__ index, int64_t rows, int64_t V, int64_t
 
 // The last kernel of a call hands its status on to the device's sticky slot.
 __device__ __forceinline__ void publish(const int* status, int* slot) {
-  if (slot && blockIdx.x == 0 && threadIdx.x == 0) {
-    const int v = *reinterpret_cast<const volatile int*>(status);
-    if (v) {
-      volatile int* h = slot;
-      *h = *h | v;
-    }
-  }
+  if (slot && blockIdx.x == 0 && threadIdx.x == 0) report_bits(slot, *reinterpret_cast<const volatile int*>(status));
 }
 
 // Logits and statistics of one or two rows: reading W once is all the time, so

@@ -64,7 +64,7 @@ __device__ __forceinline__ int64_t seq_of(const Seqs& q, int64_t t) {
 }
 
 // Offsets that decrease or leave [0, T] are reported; every access stays in
-// bounds all the same.
+// bounds all the same. Called by whole warps.
 __device__ __forceinline__ void check_offsets(const Seqs& q, int64_t i, int64_t stride) {
   if (!q.cu) return;
   int bits = 0;
@@ -73,10 +73,8 @@ __device__ __forceinline__ void check_offsets(const Seqs& q, int64_t i, int64_t 
     if (v < 0 || v > q.T || u > v) bits |= GH_DEV_BAD_SEQLENS;
     if (q.one_each && s > 0 && v != u + 1) bits |= GH_DEV_AMBIGUOUS;
   }
-  if (bits) {
-    volatile int* h = q.slot;
-    *h = *h | bits;
-  }
+  bits = __reduce_or_sync(0xffffffffu, bits);  // one report a warp at most
+  if ((threadIdx.x & 31) == 0) report_bits(q.slot, bits);
 }
 
 // f(s, a, b) for the parts [a, b) of [t0, t1) in token order: s in [0, S), or
