@@ -525,7 +525,9 @@ __device__ __forceinline__ void pref_pair(const Seqs& q, const Pref& p, int64_t 
   const double h = c.s - r.s, z = p.beta * h - p.margin;
   double l, dh;
   if (p.kind == PREF_SIGMOID) {
-    l = (1.0 - p.smooth) * softplus(-z) + p.smooth * softplus(z);
+    // a term of weight 0 may be infinite
+    l = p.smooth < 1.0 ? (1.0 - p.smooth) * softplus(-z) : 0.0;
+    if (p.smooth > 0.0) l += p.smooth * softplus(z);
     dh = p.beta * (p.smooth - sigmoid(-z));
   } else if (p.kind == PREF_HINGE) {
     l = z < 1.0 ? 1.0 - z : (z >= 1.0 ? 0.0 : z);  // NaN stays

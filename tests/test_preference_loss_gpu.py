@@ -7,6 +7,8 @@ a step of the gradient's type, hold that; sums of n terms in fp64 add
 n 2^-53 of their absolute sum.
 """
 
+import math
+
 import pytest
 import torch
 from _token_batches import HALF, batch
@@ -228,3 +230,24 @@ def test_more_than_2_to_the_31_tokens():
     want = 0.5 / (T - 1024)
     for i in (1024, (1 << 31) - 1, 1 << 31, T - 1):
         assert abs(g[i].item() - want) <= 2.0**-8 * want
+
+
+@requires_gpu
+@pytest.mark.parametrize("smooth", [0.0, 1.0])
+def test_impossible_tokens(smooth):
+    """A log-probability of -inf in one sequence of a pair: an infinite z, and the sigmoid's term
+    of weight 0 is no part of the loss."""
+    lp = torch.tensor([[-1.0, -2.0], [-1.5, -0.5], [-1.0, -3.0], [-2.0, -1.0]], device="cuda")
+    lp[2 if smooth == 0.0 else 0, 1] = -float("inf")  # z = inf, or -inf where the sign is turned
+    lp.requires_grad_(True)
+    loss, rewards = preference_loss(lp, beta=0.5, label_smoothing=smooth, reduction="sum", return_rewards=True)
+    (grad,) = torch.autograd.grad(loss, lp)
+    z = 0.5 * ((-2.0) - (-3.0))  # the second pair, without infinities
+    want = math.log1p(math.exp(-z if smooth == 0.0 else z))
+    assert abs(loss.item() - want) <= 2.0**-22 * want
+    assert (grad[::2] == 0).all()  # the first pair is decided
+    slope = 0.5 * (1 / (1 + math.exp(z)) if smooth == 0.0 else 1 / (1 + math.exp(-z)))
+    sign = 1.0 if smooth == 0.0 else -1.0
+    for row, want in ((1, -sign * slope), (3, sign * slope)):
+        assert (grad[row].double() - want).abs().amax() <= 2.0**-22 * slope
+    assert rewards.rejected[0].isinf() if smooth == 0.0 else rewards.chosen[0].isinf()
