@@ -764,7 +764,8 @@ extern "C" int gh_policy_loss_fwd(const void* logprobs, int dtype, const void* o
   if (reduction < RED_SUM || reduction > RED_SEQ_MEAN) return set_error(GH_EINVAL, "bad reduction %d", reduction);
   if (advantages_per < 0 || advantages_per > 2) return set_error(GH_EINVAL, "bad advantages_per %d", advantages_per);
   if (!(clip_low >= 0.0) || !(clip_high >= 0.0)) return set_error(GH_EINVAL, "clip bounds must not be negative");
-  if ((tokens > 0 && (!logprobs || !advantages)) || !loss || !metrics || !scal || !workspace)
+  // offsets of no sequence: per-sequence advantages are empty
+  if ((tokens > 0 && (!logprobs || (!advantages && seqs > 0))) || !loss || !metrics || !scal || !workspace)
     return set_error(GH_EINVAL, "null pointer argument");
   const PolicyLayout L = policy_layout(tokens, seqs, reduction);
   if (workspace_bytes < L.total)

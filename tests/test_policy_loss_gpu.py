@@ -333,3 +333,16 @@ def test_more_than_2_to_the_31_tokens():
     assert abs(mean.item() + 3.0) <= 8 * F
     assert abs(torch.autograd.grad(mean, lp)[0][T - 1].item() + 3.0 / T) <= 2.0**-8 * 3.0 / T
     assert g[T - 8] == 4 and (g[T - 7 :] == 0).all() and (g[100 : (1 << 31) + 5 : 4099] == -2).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("reduction", ["sum", "mean", "sequence_mean"])
+@pytest.mark.parametrize("T", [5, 20_000])
+def test_no_sequences(T, reduction):
+    """Offsets of no sequence: no token counts, and per-sequence advantages are empty."""
+    lp = torch.full((T,), float("nan"), device="cuda", requires_grad=True)
+    cu = torch.tensor([3], device="cuda")
+    for adv in (torch.empty(0, device="cuda"), torch.ones(T, device="cuda")):
+        loss, metrics = clipped_policy_loss(lp, None, adv, cu_seqlens=cu, reduction=reduction, return_metrics=True)
+        (grad,) = torch.autograd.grad(loss, lp)
+        assert loss == 0 and metrics.tokens == 0 and (grad == 0).all()
