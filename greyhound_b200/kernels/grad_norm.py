@@ -28,6 +28,16 @@ def is_dense(t: Tensor) -> bool:
     return True
 
 
+def _apart(t: Tensor) -> bool:
+    """Whether each of ``t``'s elements has memory of its own (seen from the strides, in any order)."""
+    end = 0
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride <= end:
+            return False
+        end += stride * (size - 1)
+    return True
+
+
 _CODES = {torch.float16: _lib.GH_F16, torch.bfloat16: _lib.GH_BF16, torch.float32: _lib.GH_F32}
 
 
@@ -83,7 +93,14 @@ def _operands(
         return codes, tensors, outputs, []
     src, dst = [], []
     back: list[tuple[Tensor, Tensor]] = []
-    for o, t in zip(outputs, tensors):
+    seen: dict[tuple, int] = {}  # views with gaps: the C entry compares those without
+    for i, (o, t) in enumerate(zip(outputs, tensors)):
+        if o.numel() > 0 and not is_dense(o):
+            if not _apart(o):
+                raise ValueError(f"output {i} has elements that share memory")
+            j = seen.setdefault((o.data_ptr(), o.dtype, o.shape, o.stride()), i)
+            if j != i:
+                raise ValueError(f"tensors {j} and {i} share memory that would be scaled twice")
         s = _dense(t)
         # written in place of the input's dense copy, or where input and output are laid out alike
         d = s if o is t else o if s is t and o.stride() == t.stride() else torch.empty_like(s)

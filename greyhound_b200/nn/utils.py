@@ -48,8 +48,9 @@ def clip_by_global_norm(
     ``norm`` is ``global_norm(tensors)`` before clipping. ``out`` gives the
     tensors to write, of the same shapes and types: new ones by default, or
     ``tensors`` themselves for clipping in place, which writes nothing when the
-    norm is below ``max_norm``. Outputs may not overlap each other or another
-    tensor's input (``ValueError``). A NaN norm makes every element NaN, an
+    norm is below ``max_norm``. Outputs may not overlap themselves, each other or
+    another tensor's input (``ValueError``; between views with gaps in their
+    memory only the same view listed twice is noticed). A NaN norm makes every element NaN, an
     infinite one makes finite elements 0, as the formula says; an infinite
     ``max_norm`` changes nothing.
     """

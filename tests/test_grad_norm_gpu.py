@@ -284,3 +284,16 @@ def test_within_a_compiled_function():
 
     for got, want in zip(torch.compile(scaled)(*ts), scaled(*ts)):
         assert torch.equal(got, want)
+
+
+@requires_gpu
+def test_outputs_that_overlap_themselves_are_refused_before_anything_is_written():
+    a, b = make([(300,), (40, 9)], TYPES[:1], 14)
+    wide = torch.ones(1, 7, device="cuda").expand(5, 7)
+    keep = [a.clone(), b.clone()]
+    for ts, out in (([a, wide, b], None), ([a, b, wide.contiguous()], [a, b, wide]), ([a, b[:, :5], b[:, :5]], None)):
+        with pytest.raises(ValueError, match="memory"):
+            clip_by_global_norm(ts, 0.1, out=ts if out is None else out)
+        assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
+    # as an input alone it may
+    check_clip([a, wide, b], 0.1)
