@@ -245,6 +245,8 @@ def preference_loss_forward(
         raise ValueError("label_smoothing goes with loss_type='sigmoid'")
     if ref_logprobs is not None:
         _check_like("ref_logprobs", ref_logprobs, logprobs)
+    if logprobs.ndim == 0:
+        raise ValueError("expected logprobs [sequences, length] or [tokens], got shape ()")
     if logprobs.ndim == 1 and cu_seqlens is None:
         raise ValueError("packed logprobs need cu_seqlens")
     seqs = cu_seqlens.numel() - 1 if cu_seqlens is not None and cu_seqlens.ndim == 1 else logprobs.shape[0]

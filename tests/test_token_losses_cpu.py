@@ -146,3 +146,10 @@ def test_workspaces_are_modest():
     assert lib.gh_policy_loss_workspace_bytes(1 << 22, 512, 2) < 1 << 20
     assert lib.gh_preference_loss_workspace_bytes(1 << 22, 512) < 1 << 20
     assert lib.gh_global_norm_workspace_bytes(10_000) < 1 << 20
+
+
+@pytest.mark.parametrize("kw", [{}, {"cu_seqlens": z(3, dtype=I32)}])
+def test_a_number_is_no_batch(kw):
+    for f in (lambda: pref(z(()), **kw), lambda: policy(z(()), None, z(1), **kw)):
+        with pytest.raises(ValueError, match="sequences, length|packed"):
+            f()
