@@ -79,17 +79,30 @@ __device__ __forceinline__ void check_offsets(const Seqs& q, int64_t i, int64_t 
 
 // f(s, a, b) for the parts [a, b) of [t0, t1) in token order: s in [0, S), or
 // -1 for tokens that are in no sequence. Every token comes exactly once and s
-// never repeats or decreases, also where the offsets are not in order.
+// never repeats or decreases, also where the offsets are not in order. Behind a
+// few empty sequences the next one that is not is searched for: a million of them
+// between two tokens (offsets filled up to a fixed number) cost one warp 300 ms
+// one by one. A search that offsets out of order have misled is not soon repeated.
 template <typename F>
 __device__ __forceinline__ void walk(const Seqs& q, int64_t t0, int64_t t1, F&& f) {
   int64_t cur = t0;
   int64_t s = cur < t1 ? seq_of(q, cur) : 0;
+  int empty = 0, patience = 8;
   while (cur < t1) {
     int64_t end = s >= q.S ? t1 : seq_start(q, s + 1);
     if (end > t1) end = t1;
     if (end > cur) {
       f(s >= q.S ? (int64_t)-1 : s, cur, end);
       cur = end;
+      empty = 0;
+    } else if (++empty >= patience) {
+      empty = 0;
+      const int64_t n = seq_of(q, cur);
+      if (n > s) {
+        s = n;
+        continue;
+      }
+      if (patience < 1 << 20) patience *= 2;
     }
     ++s;
   }
