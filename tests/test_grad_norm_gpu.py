@@ -297,3 +297,25 @@ def test_outputs_that_overlap_themselves_are_refused_before_anything_is_written(
         assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
     # as an input alone it may
     check_clip([a, wide, b], 0.1)
+
+
+@requires_gpu
+def test_compiled_clipping_in_place():
+    """Under torch.compile the custom ops change the tensors themselves, and the gradients."""
+    ts = make([(300,), (17, 9)], TYPES[:1], 15)
+    limit = 0.5 * norm64(ts)
+
+    def in_place(a, b):
+        a, b = a * 2.0, b * 2.0
+        _, n = clip_by_global_norm([a, b], limit, out=[a, b])
+        return a + 1.0, b + 1.0, n
+
+    def gradients(a, b):
+        p, q = torch.nn.Parameter(a), torch.nn.Parameter(b)
+        (p.square().sum() + q.square().sum()).backward()
+        n = clip_grad_norm_([p, q], limit)
+        return p.grad, q.grad, n
+
+    for f in (in_place, gradients):
+        for got, want in zip(torch.compile(f)(*ts), f(*ts)):
+            assert torch.allclose(got, want, rtol=2.0**-22, atol=0.0)
