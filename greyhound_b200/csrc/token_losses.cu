@@ -255,7 +255,8 @@ __device__ __forceinline__ Sums policy_tokens(const Seqs& q, const Policy& p, in
         float g = 0.f;
         if (on[j]) {
           const float A = av[j];
-          const float d = x[j] - y[j];
+          // without old the ratio is 1 even of 0 / 0; a NaN stays
+          const float d = olds || x[j] != x[j] ? x[j] - y[j] : 0.f;
           bool above = d > p.hi_f, below = d < p.lo_f;
           if (fabsf(d - p.hi_f) < 0x1p-16f || fabsf(d - p.lo_f) < 0x1p-16f) {
             const double e = (double)x[j] - (double)y[j];

@@ -346,3 +346,16 @@ def test_no_sequences(T, reduction):
         loss, metrics = clipped_policy_loss(lp, None, adv, cu_seqlens=cu, reduction=reduction, return_metrics=True)
         (grad,) = torch.autograd.grad(loss, lp)
         assert loss == 0 and metrics.tokens == 0 and (grad == 0).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ratio_is_one_without_old_logprobs(dtype):
+    """Also for a token of log-probability -inf; a NaN stays one."""
+    lp = torch.tensor([-1.0, -float("inf"), -3.0, 0.0], device="cuda", dtype=dtype, requires_grad=True)
+    adv = torch.tensor([1.0, -2.0, 0.5, 4.0], device="cuda")
+    loss = clipped_policy_loss(lp, None, adv, reduction="sum")
+    (grad,) = torch.autograd.grad(loss, lp)
+    assert loss == -3.5 and torch.equal(grad.float(), -adv)
+    lp = torch.tensor([-1.0, float("nan")], device="cuda", dtype=dtype)
+    assert clipped_policy_loss(lp, None, adv[:2]).isnan()
