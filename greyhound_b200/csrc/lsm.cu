@@ -22,8 +22,10 @@
 //              stored relative to its largest value, and a pass over a chunk of
 //              rows turns that into d.
 //   recomputed the backward repeats the logits GEMM row chunk by row chunk with an
-//              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, but 2 GB of
-//              workspace whatever N.
+//              epilogue that writes d (EPI_LSM_GRAD): four GEMMs, but d for one
+//              chunk of rows at a time (the caller's choice) and, over several
+//              chunks, 4 D V bytes for dW's fp32 sum, where the kept form holds
+//              2 N V bytes from one pass to the other.
 // Bound by the tensor pipe for many rows and by reading W once for few.
 #include <algorithm>
 #include <cfloat>

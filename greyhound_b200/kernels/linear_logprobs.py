@@ -28,8 +28,8 @@ __all__ = [
 
 # Largest e^x buffer held from the forward to the backward. With it a step is
 # three GEMMs, without it four and one chunk of logits' gradient: 8192 x 4096 x
-# 128256 19.5 against 26.3 ms, with the same peak of memory (one chunk), and
-# 2048 x 2048 x 100000 1.9 against 2.5 ms. 4 GiB is 16384 rows of a
+# 128256 19.1-20.2 against 26.1 ms, with the same peak of memory (one chunk), and
+# 2048 x 2048 x 100000 2.0 against 2.6 ms. 4 GiB is 16384 rows of a
 # 128256-token vocabulary, twice the logits chunk of the largest heads;
 # GREYHOUND_B200_LSM_KEEP_GB sets another limit.
 _KEEP_BYTES = int(float(os.environ.get("GREYHOUND_B200_LSM_KEEP_GB") or 4) * (1 << 30))

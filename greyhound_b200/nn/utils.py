@@ -1,8 +1,11 @@
 """Gradient norm and clipping over many tensors.
 
-``clip_grad_norm_`` takes what ``torch.nn.utils.clip_grad_norm_`` takes, without a
-host sync and in two launches; ``clip_by_global_norm`` is the form for a list of
-tensors that need not belong to parameters, in place or not.
+``clip_grad_norm_`` has the arguments of ``torch.nn.utils.clip_grad_norm_`` and works
+without a host sync, in two launches. It takes less: the 2- and the inf-norm of
+dense fp16, bf16 and fp32 gradients on one CUDA device, each with memory of its own;
+other norms, fp64, sparse or distributed gradients, several devices and shared
+gradients are refused. ``clip_by_global_norm`` is the form for a list of tensors
+that need not belong to parameters, in place or not.
 """
 
 from __future__ import annotations
